@@ -2,7 +2,7 @@
 
 * append: new keys and values rotated by their positions and appended to a paged cache, the queries rotated beside them
   (`capi.rope_append`), into 16-bit caches and into the 8-bit cache with one scale per block and kv head;
-* attend: paged attention over that 8-bit cache (`capi.paged_attention` with cache type I8);
+* attend: paged attention over that 8-bit cache (`capi.paged_attention_i8`);
 * product: a projection with 8-bit weights, a scale per output channel, on activations of 8 bits with a scale per token
   (`ops_capi.matmul_i8`), which come as they are or are quantised on the way in (`ops_capi.quantize_rows`), behind an RMS
   norm or a GLU where the layer has one there.
@@ -213,14 +213,14 @@ def _prepare_append(case, gen):
     s["q_out"] = torch.empty((T, H * D), device="cuda", dtype=dtype)
     if own:
         from openvino_contrib_amd import capi
-        scales = [s[n].data_ptr() if s[n] is not None else None for n in ("key_scales", "value_scales")]
         s["desc"] = capi.PaDesc(code, code, TYPES[case["cache"]][0], code, H, K, D, case["block"], s["blocks"], T, len(s["seqs"]), s["longest"],
-                                0, 0.0, 0, 0, None, None, *scales)
+                                0, 0.0, 0, 0, None, None)
         s["rope"] = capi.RopeAppendDesc(table_dtype=0, rotary_ndims=R, interleaved=int(case["interleaved"]), table_rows=s["longest"],
                                         table_row_stride=s["cos"].shape[1], q_token_stride=s["q"].stride(0), k_token_stride=s["k"].stride(0),
                                         v_token_stride=s["v"].stride(0), q_out_token_stride=H * D)
-        s["args"] = [Buffer(s[n]) for n in ("q", "k", "v", "cos", "sin")] + [None] + [
-            Buffer(s[n]) for n in ("q_out", "keys", "values", "past", "begins", "table", "table_begins")]
+        s["positions"] = None  # the tokens' places in the cache
+        s["args"] = [Buffer(s[n]) if s[n] is not None else None for n in ("q", "k", "v", "cos", "sin", "positions", "q_out", "keys", "values",
+                     "key_scales", "value_scales", "past", "begins", "table", "table_begins")]
     return s
 
 
@@ -233,11 +233,10 @@ def _prepare_attend(case, gen):
     if own:
         from openvino_contrib_amd import capi
         s["desc"] = capi.PaDesc(code, code, TYPES["i8"][0], code, H, K, D, case["block"], s["blocks"], T, len(s["seqs"]), s["longest"],
-                                case["window"], 0.0, capi.PA_SKIP_CACHE_WRITE, 0, None, None, s["key_scales"].data_ptr(),
-                                s["value_scales"].data_ptr())
+                                case["window"], 0.0, capi.PA_SKIP_CACHE_WRITE, 0, None, None)
         s["workspace"] = torch.empty(max(16, capi.paged_attention_workspace_size(s["desc"])), device="cuda", dtype=torch.uint8)
-        s["args"] = [Buffer(s["q"]), None, None] + [Buffer(s[n]) for n in ("keys", "values", "past", "begins", "table", "table_begins", "out",
-                                                                        "workspace")]
+        s["args"] = [Buffer(s["q"]), None, None] + [Buffer(s[n]) for n in ("keys", "values", "key_scales", "value_scales", "past", "begins",
+                                                                        "table", "table_begins", "out", "workspace")]
     return s
 
 
@@ -407,7 +406,7 @@ def run(state):
     if case["path"] == "attend":
         if own:
             from openvino_contrib_amd import capi
-            capi.paged_attention(state["desc"], *state["args"])
+            capi.paged_attention_i8(state["desc"], *state["args"])
         else:
             _plain_part(state, case, 0, case["prompts"])
             _plain_part(state, case, case["prompts"], len(state["seqs"]))
