@@ -39,7 +39,8 @@ typedef enum hipattn_dtype {
     HIPATTN_F32 = 0,
     HIPATTN_F16 = 1,
     HIPATTN_BF16 = 2,
-    HIPATTN_U8 = 3 /* KV cache only: rows of [scale f32][zero-point f32][head_dim bytes] */
+    HIPATTN_U8 = 3, /* KV cache only: rows of [scale f32][zero-point f32][head_dim bytes] */
+    HIPATTN_I8 = 4  /* KV cache only: rows of head_dim signed bytes, one f32 scale per (block, kv head) in arrays of their own */
 } hipattn_dtype;
 
 typedef struct hipattn_stream_t* hipattn_stream; /* a hipStream_t; NULL is the default stream */
@@ -172,7 +173,8 @@ hipattn_status hipattn_sdpa_masked(const hipattn_sdpa_desc* desc, const void* q,
  *   k_new, v_new          [num_tokens, num_heads_kv * head_dim]             kv_dtype
  *   key_cache,value_cache [num_blocks, num_heads_kv, block_size, row]       cache_dtype
  *                         row = head_dim elements, or for HIPATTN_U8
- *                         [scale f32][zero-point f32][head_dim bytes] per token and head
+ *                         [scale f32][zero-point f32][head_dim bytes] per token and head,
+ *                         or for HIPATTN_I8 head_dim signed bytes (hipattn_paged_attention_i8)
  *   past_lens             [num_seqs] i32      tokens already cached per sequence
  *   subsequence_begins    [num_seqs + 1] i32  token offsets of each sequence in this batch
  *   block_indices         [...] i32           physical block ids, sequence after sequence
@@ -318,6 +320,62 @@ hipattn_status hipattn_rotate_key_cache(const hipattn_pa_desc* desc, void* key_c
                                         const int32_t* rotation_deltas, int deltas_per_block,
                                         const void* rotation_trig_lut, int lut_dtype, int lut_rows,
                                         hipattn_stream stream);
+
+/* PagedAttentionExtension over a cache of type HIPATTN_I8: rows of head_dim signed bytes, and for each block and kv head one
+ * scale, value = scale * code.  key_scales and value_scales are device arrays [num_blocks, num_heads_kv] of floats, kept
+ * beside the caches; everything else is as in hipattn_paged_attention (which refuses this type, having no place for
+ * them), and so is the workspace (hipattn_paged_attention_workspace_size).  No counterpart in the reference.
+ * The calls that write such a cache (this one without HIPATTN_PA_SKIP_CACHE_WRITE, and hipattn_rope_append) keep the scales up to
+ * date.  With a = the largest magnitude among the rows that one call writes into the block for the head,
+ *     scale' = max(scale before, a / 127)      (scale before: 0 when the call writes the block's row 0; a / 127 below 1e-30: 0)
+ *     code   = clamp(rint(x * (1 / scale')), -127, 127)                              for the new rows
+ *     code'  = rint(code * (scale before / scale'))       for the rows that precede them, when the scale has grown
+ * in fp32, every operation rounded by itself; codes are 0 where the scale is.  Rows behind the new ones keep their bytes.
+ * Repeating a call changes nothing.  New rows that hold infinities or NaN leave their block's values undefined.
+ * 16-bit queries with a head_dim that is a multiple of 16 up to 128 on blocks of 16, 32 or a larger power of two, and at
+ * most 16 query heads per kv head or groups of 8 to 16, take the matrix-core kernels; the rest, sinks and alibi_slopes
+ * among it, the shape-generic kernels.  The scores output and the cache rotation refuse this type. */
+hipattn_status hipattn_paged_attention_i8(const hipattn_pa_desc* desc, const void* q, const void* k_new, const void* v_new,
+                                          void* key_cache, void* value_cache, float* key_scales, float* value_scales,
+                                          const int32_t* past_lens, const int32_t* subsequence_begins,
+                                          const int32_t* block_indices, const int32_t* block_indices_begins, void* out,
+                                          void* workspace, size_t workspace_bytes, hipattn_stream stream);
+
+/* Step 1 with the rotary position embedding applied on the way: what a decoder layer does between its q / k / v projection
+ * and its attention, in one launch.  No counterpart in the reference, whose chain is hipops_rope's (src/ops/strided_slice.cpp,
+ * src/ops/concat.cpp:20-102, src/ops/multiply.cpp:43, src/ops/add.cpp:17-43) and a copy of the variable state.
+ *
+ * Token t of sequence s stands at position p = past_lens[s] + t - subsequence_begins[s].  The first rotary_ndims elements of each
+ * query and key head are turned by the table's row (positions[t] when positions is not NULL, else p), in the two layouts of
+ * hipops_rope (rotate-half tables have rotary_ndims columns, interleaved ones rotary_ndims / 2); products and the sum are
+ * fp32, each rounded by itself, and are rounded once more to the type of q_out or stored in the cache straight from
+ * fp32 -- converted, or quantised (HIPATTN_U8 as by hipattn_kv_cache_write, HIPATTN_I8 as described at hipattn_paged_attention_i8).  Values
+ * are stored as they are.  Tokens whose row lies outside [0, table_rows), and tokens outside every sequence, are not turned;
+ * tokens whose cache position has no block are not stored, as in hipattn_paged_attention.
+ *
+ * q, k_new, v_new, q_out: element i of head h of token t at t * token_stride + h * head_stride + i, in elements; a stride of 0
+ * stands for packed rows (head_stride = head_dim, token_stride = heads * head_dim), so the three may be slices of one
+ * projection.  q and q_out may both be NULL (append alone), and may be one array with equal strides (in place); cos and sin
+ * may both be NULL (no rotation).  Of desc: q_dtype (q and q_out), kv_dtype, cache_dtype, the heads, head_dim, block_size,
+ * num_blocks, num_tokens and num_seqs; blocks that this call writes belong to one sequence.  key_scales and value_scales: the
+ * scales of an i8 cache, else NULL.
+ * 16-bit q, k_new and v_new of one type at multiples of 16 bytes, with head_dim and rotary_ndims multiples of 16, take the
+ * vector form; everything else the scalar one. */
+typedef struct hipattn_rope_append_desc {
+    int table_dtype;  /* cos and sin: F32 / F16 / BF16 */
+    int rotary_ndims; /* even, <= head_dim; 0 selects head_dim */
+    int interleaved;
+    int table_rows;
+    int64_t table_row_stride;
+    int64_t q_token_stride, k_token_stride, v_token_stride, q_out_token_stride;
+    int64_t q_head_stride, k_head_stride, v_head_stride, q_out_head_stride;
+} hipattn_rope_append_desc;
+hipattn_status hipattn_rope_append(const hipattn_pa_desc* desc, const hipattn_rope_append_desc* rope_desc, const void* q,
+                                   const void* k_new, const void* v_new, const void* cos, const void* sin,
+                                   const int32_t* positions, void* q_out, void* key_cache, void* value_cache,
+                                   float* key_scales, float* value_scales, const int32_t* past_lens,
+                                   const int32_t* subsequence_begins, const int32_t* block_indices,
+                                   const int32_t* block_indices_begins, hipattn_stream stream);
 
 /* Step 1 alone: the device-side KV-cache block writer. */
 hipattn_status hipattn_kv_cache_write(const hipattn_pa_desc* desc, const void* k_new, const void* v_new,

@@ -17,6 +17,7 @@ LIB_PATH = os.path.join(CSRC, "libhipattn.so")
 SOURCES = [
     "hipattn_api.hip",
     "kv_cache_write.hip",
+    "rope_append.hip",
     "attention_generic.hip",
     "sdpa_f32.hip",
     "sdpa_narrow.hip",

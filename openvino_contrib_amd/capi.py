@@ -13,12 +13,12 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "csrc", "libhipattn.so")
 
 OK, INVALID_ARGUMENT, UNSUPPORTED, WORKSPACE_TOO_SMALL, HIP_ERROR, NO_DEVICE = range(6)
-F32, F16, BF16, U8 = 0, 1, 2, 3
+F32, F16, BF16, U8, I8 = 0, 1, 2, 3, 4
 PA_SKIP_CACHE_WRITE = 1
 PA_FORCE_GENERIC = 2
 PA_ANY_LENGTHS = 8
 
-DTYPE_BYTES = {F32: 4, F16: 2, BF16: 2, U8: 1}
+DTYPE_BYTES = {F32: 4, F16: 2, BF16: 2, U8: 1, I8: 1}
 
 
 class HipAttnError(RuntimeError):
@@ -83,6 +83,24 @@ class PaDesc(ctypes.Structure):
     ]
 
 
+class RopeAppendDesc(ctypes.Structure):
+    _fields_ = [
+        ("table_dtype", ctypes.c_int),
+        ("rotary_ndims", ctypes.c_int),
+        ("interleaved", ctypes.c_int),
+        ("table_rows", ctypes.c_int),
+        ("table_row_stride", ctypes.c_int64),
+        ("q_token_stride", ctypes.c_int64),
+        ("k_token_stride", ctypes.c_int64),
+        ("v_token_stride", ctypes.c_int64),
+        ("q_out_token_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("v_head_stride", ctypes.c_int64),
+        ("q_out_head_stride", ctypes.c_int64),
+    ]
+
+
 # every symbol include/hipattn.h declares: name -> (restype, argtypes)
 _vp, _i, _sz, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_float
 _P = ctypes.POINTER
@@ -125,6 +143,8 @@ SYMBOLS = {
     "hipattn_paged_attention_scores_workspace_size": (_i, [_P(PaDesc), _P(_sz)]),
     "hipattn_paged_attention_scores": (_i, [_P(PaDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_int64, _vp, _sz, _vp]),
     "hipattn_set_option": (_i, [ctypes.c_char_p, _i]),
+    "hipattn_rope_append": (_i, [_P(PaDesc), _P(RopeAppendDesc)] + [_vp] * 16),
+    "hipattn_paged_attention_i8": (_i, [_P(PaDesc)] + [_vp] * 13 + [_sz, _vp]),
     "hipattn_kv_cache_write": (_i, [_P(PaDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "hipattn_rotate_key_cache": (_i, [_P(PaDesc), _vp, _vp, _i, _vp, _i, _vp, _i, _i, _vp]),
     "hipattn_cache_row_bytes": (_sz, [_i, _i]),
@@ -304,6 +324,15 @@ def paged_attention(desc, q, k_new, v_new, key_cache, value_cache, past_lens, su
         out.ptr, workspace.ptr if workspace else None, workspace.nbytes if workspace else 0, _h(stream)))
 
 
+def paged_attention_i8(desc, q, k_new, v_new, key_cache, value_cache, key_scales, value_scales, past_lens, subsequence_begins,
+                       block_indices, block_indices_begins, out, workspace=None, stream=None):
+    """Attention over a cache of type I8, whose scales [num_blocks, num_heads_kv] lie beside it."""
+    bufs = (q, k_new, v_new, key_cache, value_cache, key_scales, value_scales, past_lens, subsequence_begins, block_indices,
+            block_indices_begins, out, workspace)
+    check(lib().hipattn_paged_attention_i8(ctypes.byref(desc), *[b.ptr if b is not None else None for b in bufs],
+                                           workspace.nbytes if workspace is not None else 0, _h(stream)))
+
+
 def paged_attention_noalloc(desc, q, k_new, v_new, key_cache, value_cache, past_lens, subsequence_begins,
                             block_indices, block_indices_begins, out, stream=None):
     """The entry point that allocates nothing: scratch is the library's static device array."""
@@ -342,6 +371,15 @@ def rotate_key_cache(desc, key_cache, rotated_block_indices, rotation_deltas, de
     n = rotated_block_indices.nbytes // 4
     check(lib().hipattn_rotate_key_cache(ctypes.byref(desc), key_cache.ptr, rotated_block_indices.ptr, n, rotation_deltas.ptr,
                                          deltas_per_block, trig_lut.ptr, lut_dtype, lut_rows, _h(stream)))
+
+
+def rope_append(desc, rope_desc, q, k_new, v_new, cos, sin, positions, q_out, key_cache, value_cache, key_scales, value_scales, past_lens,
+                subsequence_begins, block_indices, block_indices_begins, stream=None):
+    """New keys and values into the caches, rotated on the way, and the queries rotated beside them; q with q_out, cos with sin,
+    positions, and the scales of a cache that is not I8 may be None."""
+    bufs = (q, k_new, v_new, cos, sin, positions, q_out, key_cache, value_cache, key_scales, value_scales, past_lens, subsequence_begins,
+            block_indices, block_indices_begins)
+    check(lib().hipattn_rope_append(ctypes.byref(desc), ctypes.byref(rope_desc), *[b.ptr if b is not None else None for b in bufs], _h(stream)))
 
 
 def kv_cache_write(desc, k_new, v_new, key_cache, value_cache, past_lens, subsequence_begins, block_indices,

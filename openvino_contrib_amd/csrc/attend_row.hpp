@@ -35,7 +35,7 @@ struct MaskRow {
 };
 
 // Attend one query row to keys [j0, j1).  q_row is the row in fp32 (LDS or global memory); KV yields row
-// pointers and says which keys exist (a key in a block outside the cache has probability zero);
+// pointers, what their elements are still to be multiplied by, and says which keys exist (a key in a block outside the cache has probability zero);
 // bias(j) is added to the scaled score of key j.  Every lane of the wavefront must call this; the
 // result for head-dim slot d = lane + 64 * i < 64 * kSlots is returned in o[i], already normalised.  A row that
 // can attend nothing (empty range, every key masked with -inf) yields zeros.
@@ -55,7 +55,7 @@ __device__ __forceinline__ void attend_row_wave(const float* q_row, const KV& kv
             const uint8_t* krow = kv.k_row(j);
             float acc = 0.0f;
             for (int d = 0; d < D; d++) acc = fmaf(q_row[d], load_cache_elem(krow, d, kv.dtype), acc);
-            s = fmaf(acc, c, bias(j) * kLog2e);
+            s = fmaf(acc * kv.k_scale(j), c, bias(j) * kLog2e);
         }
         const float m_new = fmaxf(m, wave_max(s));
         if (m_new == -INFINITY) continue;  // nothing attended so far (wave-uniform)
@@ -67,9 +67,10 @@ __device__ __forceinline__ void attend_row_wave(const float* q_row, const KV& kv
         for (int i = 0; i < kSlots; i++) o[i] *= alpha;
         const int n = min(64, j1 - base);
         for (int jj = 0; jj < n; jj++) {
-            const float pb = __shfl(pj, jj, 64);
+            float pb = __shfl(pj, jj, 64);
             if (pb == 0.0f) continue;  // (wave-uniform) masked keys may be unreadable or hold anything
             const uint8_t* vrow = kv.v_row(base + jj);
+            pb *= kv.v_scale(base + jj);
 #pragma unroll
             for (int i = 0; i < kSlots; i++) {
                 const int d = lane + 64 * i;
@@ -91,6 +92,8 @@ struct DenseKV {
     __device__ __forceinline__ bool exists(int) const { return true; }
     __device__ __forceinline__ const uint8_t* k_row(int j) const { return k + j * row_bytes; }
     __device__ __forceinline__ const uint8_t* v_row(int j) const { return v + j * row_bytes; }
+    static __device__ __forceinline__ float k_scale(int) { return 1.0f; }
+    static __device__ __forceinline__ float v_scale(int) { return 1.0f; }
 };
 
 }  // namespace hipattn

@@ -22,6 +22,9 @@ struct PagedKV {
     int block_size;
     int dtype;
     int num_blocks;
+    const float* k_scales;  // HIPATTN_I8: scales of this kv head, num_heads_kv apart; nullptr otherwise
+    const float* v_scales;
+    int num_heads_kv;
     // a block id outside the cache: its keys are skipped (probability zero), as the decode kernel does
     __device__ __forceinline__ bool exists(int j) const {
         const int pb = blocks[j / block_size];
@@ -32,6 +35,12 @@ struct PagedKV {
     }
     __device__ __forceinline__ const uint8_t* k_row(int j) const { return k + off(j); }
     __device__ __forceinline__ const uint8_t* v_row(int j) const { return v + off(j); }
+    __device__ __forceinline__ float k_scale(int j) const {
+        return k_scales ? k_scales[(int64_t)blocks[j / block_size] * num_heads_kv] : 1.0f;
+    }
+    __device__ __forceinline__ float v_scale(int j) const {
+        return v_scales ? v_scales[(int64_t)blocks[j / block_size] * num_heads_kv] : 1.0f;
+    }
 };
 
 __global__ __launch_bounds__(64 * kWavesPerBlock) void sdpa_generic_kernel(SdpaParams p) {
@@ -105,7 +114,10 @@ __global__ __launch_bounds__(64 * kWavesPerBlock) void paged_generic_kernel(Page
                (int64_t)(h / G) * p.block_size * rb,
                p.block_size,
                p.cache_dtype,
-               p.num_blocks};
+               p.num_blocks,
+               p.cache_dtype == HIPATTN_I8 ? p.key_scales + h / G : nullptr,
+               p.cache_dtype == HIPATTN_I8 ? p.value_scales + h / G : nullptr,
+               p.num_heads_kv};
     // never read beyond the sequence's block table
     const int table_tokens = (p.block_indices_begins[s + 1] - p.block_indices_begins[s]) * p.block_size;
     const int j1 = min(pos + 1, table_tokens);

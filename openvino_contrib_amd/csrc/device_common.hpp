@@ -104,7 +104,7 @@ __device__ __forceinline__ void store_scalar(void* base, int64_t idx, int dtype,
 }
 
 __host__ __device__ __forceinline__ int dtype_bytes(int dtype) {
-    return dtype == HIPATTN_F32 ? 4 : (dtype == HIPATTN_U8 ? 1 : 2);
+    return dtype == HIPATTN_F32 ? 4 : (dtype == HIPATTN_U8 || dtype == HIPATTN_I8 ? 1 : 2);
 }
 
 __host__ __device__ __forceinline__ int64_t cache_row_bytes(int cache_dtype, int head_dim) {
@@ -112,16 +112,18 @@ __host__ __device__ __forceinline__ int64_t cache_row_bytes(int cache_dtype, int
         case HIPATTN_F32: return 4 * (int64_t)head_dim;
         case HIPATTN_F16:
         case HIPATTN_BF16: return 2 * (int64_t)head_dim;
+        case HIPATTN_I8: return (int64_t)head_dim;
         default: return (int64_t)head_dim + 8;
     }
 }
 
-// one element of a cache row, dequantised
+// one element of a cache row, dequantised (i8: the code; its scale is the block's)
 __device__ __forceinline__ float load_cache_elem(const uint8_t* row, int d, int cache_dtype) {
     switch (cache_dtype) {
         case HIPATTN_F32: return ((const float*)row)[d];
         case HIPATTN_F16: return f16_bits_to_float(((const uint16_t*)row)[d]);
         case HIPATTN_BF16: return bf16_bits_to_float(((const uint16_t*)row)[d]);
+        case HIPATTN_I8: return (float)(int8_t)row[d];
         default: {
             float scale = ((const float*)row)[0];
             float zp = ((const float*)row)[1];

@@ -64,7 +64,7 @@ hipattn_status validate_pa(const hipattn_pa_desc* d, bool need_q) {
     if (!d) return fail(HIPATTN_INVALID_ARGUMENT, "paged_attention: null descriptor");
     if (need_q && (!is_float_dtype(d->q_dtype) || !is_float_dtype(d->out_dtype)))
         return fail(HIPATTN_INVALID_ARGUMENT, "paged_attention: q/out dtype must be f32/f16/bf16");
-    if (!is_float_dtype(d->cache_dtype) && d->cache_dtype != HIPATTN_U8)
+    if (!is_float_dtype(d->cache_dtype) && d->cache_dtype != HIPATTN_U8 && d->cache_dtype != HIPATTN_I8)
         return fail(HIPATTN_INVALID_ARGUMENT, "paged_attention: cache dtype %d", d->cache_dtype);
     if (!(d->flags & HIPATTN_PA_SKIP_CACHE_WRITE) && !is_float_dtype(d->kv_dtype))
         return fail(HIPATTN_INVALID_ARGUMENT, "paged_attention: kv dtype %d", d->kv_dtype);
@@ -109,6 +109,35 @@ hipattn::KvWriteParams make_write_params(const hipattn_pa_desc* d, const void* k
     w.block_size = d->block_size;
     w.num_blocks = d->num_blocks;
     return w;
+}
+
+// An append without rotation and queries: what writes an i8 cache for the calls that take packed new rows.
+hipattn::RopeAppendParams make_append_params(const hipattn_pa_desc* d, const hipattn::KvWriteParams& w, float* key_scales, float* value_scales) {
+    hipattn::RopeAppendParams p{};
+    p.k_new = w.k_new;
+    p.v_new = w.v_new;
+    p.key_cache = w.key_cache;
+    p.value_cache = w.value_cache;
+    p.key_scales = key_scales;
+    p.value_scales = value_scales;
+    p.past_lens = w.past_lens;
+    p.subsequence_begins = w.subsequence_begins;
+    p.block_indices = w.block_indices;
+    p.block_indices_begins = w.block_indices_begins;
+    p.q_head = p.k_head = p.v_head = p.out_head = d->head_dim;
+    p.q_token = p.out_token = (int64_t)d->num_heads_q * d->head_dim;
+    p.k_token = p.v_token = (int64_t)d->num_heads_kv * d->head_dim;
+    p.q_dtype = d->q_dtype;
+    p.kv_dtype = d->kv_dtype;
+    p.cache_dtype = d->cache_dtype;
+    p.num_heads_q = d->num_heads_q;
+    p.num_heads_kv = d->num_heads_kv;
+    p.head_dim = d->head_dim;
+    p.block_size = d->block_size;
+    p.num_blocks = d->num_blocks;
+    p.num_tokens = d->num_tokens;
+    p.num_seqs = d->num_seqs;
+    return p;
 }
 
 hipattn::PagedParams make_paged_params(const hipattn_pa_desc* d) {
@@ -178,6 +207,7 @@ HIPATTN_EXPORT size_t hipattn_cache_row_bytes(hipattn_dtype cache_dtype, int hea
         case HIPATTN_F16:
         case HIPATTN_BF16: return 2 * (size_t)head_dim;
         case HIPATTN_U8: return (size_t)head_dim + 8;
+        case HIPATTN_I8: return (size_t)head_dim;
     }
     return 0;
 }
@@ -453,6 +483,7 @@ HIPATTN_EXPORT hipattn_status hipattn_kv_cache_write(const hipattn_pa_desc* desc
                                                      const int32_t* block_indices_begins, hipattn_stream stream) {
     if (hipattn_status st = validate_pa(desc, false)) return st;
     if (!is_float_dtype(desc->kv_dtype)) return fail(HIPATTN_INVALID_ARGUMENT, "kv_cache_write: kv dtype %d", desc->kv_dtype);
+    if (desc->cache_dtype == HIPATTN_I8) return fail(HIPATTN_UNSUPPORTED, "kv_cache_write: an i8 cache has scales beside it (hipattn_rope_append)");
     if (desc->num_tokens == 0 || desc->num_seqs == 0) return HIPATTN_OK;
     if (!k_new || !v_new || !key_cache || !value_cache || !past_lens || !subsequence_begins || !block_indices ||
         !block_indices_begins)
@@ -463,12 +494,75 @@ HIPATTN_EXPORT hipattn_status hipattn_kv_cache_write(const hipattn_pa_desc* desc
     return HIPATTN_OK;
 }
 
+HIPATTN_EXPORT hipattn_status hipattn_rope_append(const hipattn_pa_desc* desc, const hipattn_rope_append_desc* rope_desc, const void* q,
+                                                  const void* k_new, const void* v_new, const void* cos, const void* sin,
+                                                  const int32_t* positions, void* q_out, void* key_cache, void* value_cache,
+                                                  float* key_scales, float* value_scales, const int32_t* past_lens,
+                                                  const int32_t* subsequence_begins,
+                                                  const int32_t* block_indices, const int32_t* block_indices_begins,
+                                                  hipattn_stream stream) {
+    if (hipattn_status st = validate_pa(desc, false)) return st;
+    if (!rope_desc) return fail(HIPATTN_INVALID_ARGUMENT, "rope_append: null descriptor");
+    const hipattn_rope_append_desc& r = *rope_desc;
+    if (!is_float_dtype(desc->kv_dtype)) return fail(HIPATTN_INVALID_ARGUMENT, "rope_append: kv dtype %d", desc->kv_dtype);
+    if ((q == nullptr) != (q_out == nullptr)) return fail(HIPATTN_INVALID_ARGUMENT, "rope_append: q and q_out are both NULL or both set");
+    if ((cos == nullptr) != (sin == nullptr)) return fail(HIPATTN_INVALID_ARGUMENT, "rope_append: cos and sin are both NULL or both set");
+    if (q && !is_float_dtype(desc->q_dtype)) return fail(HIPATTN_INVALID_ARGUMENT, "rope_append: q dtype %d", desc->q_dtype);
+    const int rotary = r.rotary_ndims == 0 ? desc->head_dim : r.rotary_ndims;
+    if (cos) {
+        if (!is_float_dtype(r.table_dtype)) return fail(HIPATTN_INVALID_ARGUMENT, "rope_append: table dtype %d", r.table_dtype);
+        if (rotary < 0 || rotary % 2 || rotary > desc->head_dim)
+            return fail(HIPATTN_INVALID_ARGUMENT, "rope_append: rotary_ndims %d (even, at most head_dim %d)", rotary, desc->head_dim);
+        if (r.table_rows < 0 || r.table_row_stride < (r.interleaved ? rotary / 2 : rotary))
+            return fail(HIPATTN_INVALID_ARGUMENT, "rope_append: a table of %d rows, %lld apart", r.table_rows, (long long)r.table_row_stride);
+    }
+    const int64_t strides[8] = {r.q_token_stride, r.k_token_stride, r.v_token_stride, r.q_out_token_stride,
+                                r.q_head_stride,  r.k_head_stride,  r.v_head_stride,  r.q_out_head_stride};
+    for (int64_t s : strides)
+        if (s < 0) return fail(HIPATTN_INVALID_ARGUMENT, "rope_append: negative stride");
+    // (rows that share elements would be written by several wavefronts at once)
+    const int64_t out_head = r.q_out_head_stride ? r.q_out_head_stride : desc->head_dim;
+    const int64_t out_token = r.q_out_token_stride ? r.q_out_token_stride : (int64_t)desc->num_heads_q * desc->head_dim;
+    const bool by_token = out_token >= (desc->num_heads_q - 1) * out_head + desc->head_dim && out_head >= desc->head_dim;
+    const bool by_head = out_head >= (int64_t)(desc->num_tokens - 1) * out_token + desc->head_dim && out_token >= desc->head_dim;
+    if (q_out && !by_token && !by_head) return fail(HIPATTN_INVALID_ARGUMENT, "rope_append: rows of q_out overlap");
+    if (desc->num_tokens == 0 || desc->num_seqs == 0) return HIPATTN_OK;
+    if (!k_new || !v_new || !key_cache || !value_cache || !past_lens || !subsequence_begins || !block_indices || !block_indices_begins)
+        return fail(HIPATTN_INVALID_ARGUMENT, "rope_append: null pointer");
+    if (desc->cache_dtype == HIPATTN_I8 && (!key_scales || !value_scales))
+        return fail(HIPATTN_INVALID_ARGUMENT, "rope_append: an i8 cache needs key_scales and value_scales");
+    const hipattn::KvWriteParams w = make_write_params(desc, k_new, v_new, key_cache, value_cache, past_lens, subsequence_begins,
+                                                       block_indices, block_indices_begins);
+    hipattn::RopeAppendParams p = make_append_params(desc, w, key_scales, value_scales);
+    p.q = q;
+    p.q_out = q_out;
+    p.cos = cos;
+    p.sin = sin;
+    p.positions = positions;
+    p.table_dtype = r.table_dtype;
+    p.table_rows = r.table_rows;
+    p.table_row_stride = r.table_row_stride;
+    p.rotary = cos ? rotary : 0;
+    p.interleaved = r.interleaved != 0;
+    if (r.q_token_stride) p.q_token = r.q_token_stride;
+    if (r.k_token_stride) p.k_token = r.k_token_stride;
+    if (r.v_token_stride) p.v_token = r.v_token_stride;
+    if (r.q_head_stride) p.q_head = r.q_head_stride;
+    if (r.k_head_stride) p.k_head = r.k_head_stride;
+    if (r.v_head_stride) p.v_head = r.v_head_stride;
+    p.out_token = out_token;
+    p.out_head = out_head;
+    HIP_TRY(hipattn::launch_rope_append(p, as_stream(stream)));
+    return HIPATTN_OK;
+}
+
 HIPATTN_EXPORT hipattn_status hipattn_rotate_key_cache(const hipattn_pa_desc* desc, void* key_cache,
                                                        const int32_t* rotated_block_indices, int num_rotated_blocks,
                                                        const int32_t* rotation_deltas, int deltas_per_block,
                                                        const void* rotation_trig_lut, int lut_dtype, int lut_rows,
                                                        hipattn_stream stream) {
     if (hipattn_status st = validate_pa(desc, false)) return st;
+    if (desc->cache_dtype == HIPATTN_I8) return fail(HIPATTN_UNSUPPORTED, "rotate_key_cache: no rotation of i8 caches");
     if (num_rotated_blocks < 0 || lut_rows < 0) return fail(HIPATTN_INVALID_ARGUMENT, "rotate_key_cache: negative count");
     if (num_rotated_blocks == 0) return HIPATTN_OK;
     if (!key_cache || !rotated_block_indices || !rotation_deltas || !rotation_trig_lut)
@@ -515,13 +609,17 @@ hipattn_status paged_attention_impl(const hipattn_pa_desc* desc, const void* q, 
                                     void* key_cache, void* value_cache, const int32_t* past_lens,
                                     const int32_t* subsequence_begins, const int32_t* block_indices,
                                     const int32_t* block_indices_begins, void* out, void* workspace,
-                                    size_t workspace_bytes, hipattn_stream stream, bool static_scratch) {
+                                    size_t workspace_bytes, hipattn_stream stream, bool static_scratch,
+                                    float* key_scales = nullptr, float* value_scales = nullptr) {
     if (hipattn_status st = validate_pa(desc, true)) return st;
+    const bool i8 = desc->cache_dtype == HIPATTN_I8;
     if (desc->num_tokens == 0 || desc->num_seqs == 0) return HIPATTN_OK;
+    if (i8 && (!key_scales || !value_scales))
+        return fail(HIPATTN_INVALID_ARGUMENT, "paged_attention: an i8 cache needs its scales (hipattn_paged_attention_i8)");
     if (!q || !out || !key_cache || !value_cache || !past_lens || !subsequence_begins || !block_indices ||
         !block_indices_begins)
         return fail(HIPATTN_INVALID_ARGUMENT, "paged_attention: null pointer");
-    const bool do_write = !(desc->flags & HIPATTN_PA_SKIP_CACHE_WRITE);
+    bool do_write = !(desc->flags & HIPATTN_PA_SKIP_CACHE_WRITE);
     if (do_write && (!k_new || !v_new)) return fail(HIPATTN_INVALID_ARGUMENT, "paged_attention: null k_new/v_new");
     hipattn::KvWriteParams w = make_write_params(desc, k_new, v_new, key_cache, value_cache, past_lens,
                                                  subsequence_begins, block_indices, block_indices_begins);
@@ -529,6 +627,8 @@ hipattn_status paged_attention_impl(const hipattn_pa_desc* desc, const void* q, 
     p.q = q;
     p.key_cache = (const uint8_t*)key_cache;
     p.value_cache = (const uint8_t*)value_cache;
+    p.key_scales = key_scales;
+    p.value_scales = value_scales;
     p.past_lens = past_lens;
     p.subsequence_begins = subsequence_begins;
     p.block_indices = block_indices;
@@ -556,9 +656,15 @@ hipattn_status paged_attention_impl(const hipattn_pa_desc* desc, const void* q, 
         return HIPATTN_OK;
     };
     const bool forced_generic = (desc->flags & HIPATTN_PA_FORCE_GENERIC) != 0;
+    const auto write_i8 = [&]() -> hipError_t {  // a launch of its own: a block's scale needs all rows that go into it
+        if (!i8 || !do_write) return hipSuccess;
+        do_write = false;
+        return hipattn::launch_rope_append(make_append_params(desc, w, key_scales, value_scales), as_stream(stream));
+    };
     if (!forced_generic && hipattn::paged_fast_supported(p)) {
         if (hipattn_status st = take_workspace(hipattn::paged_fast_workspace_bytes(p))) return st;
         hipattn::paged_fast_plan(p, workspace, workspace_bytes);
+        HIP_TRY(write_i8());
         g_kernel_path = "paged_mfma";
         HIP_TRY(hipattn::launch_paged_fast(p, do_write ? &w : nullptr, as_stream(stream), g_probe));
     } else if (!forced_generic && hipattn::paged_tiles_supported(p)) {
@@ -568,6 +674,7 @@ hipattn_status paged_attention_impl(const hipattn_pa_desc* desc, const void* q, 
         HIP_TRY(hipattn::launch_paged_tiles(p, workspace, as_stream(stream), g_probe));
     } else {
         g_kernel_path = "paged_generic";
+        HIP_TRY(write_i8());
         if (do_write) HIP_TRY(hipattn::launch_kv_cache_write(w, as_stream(stream)));
         HIP_TRY(hipattn::launch_paged_generic(p, as_stream(stream)));
     }
@@ -583,6 +690,16 @@ HIPATTN_EXPORT hipattn_status hipattn_paged_attention(const hipattn_pa_desc* des
                                                       size_t workspace_bytes, hipattn_stream stream) {
     return paged_attention_impl(desc, q, k_new, v_new, key_cache, value_cache, past_lens, subsequence_begins,
                                 block_indices, block_indices_begins, out, workspace, workspace_bytes, stream, false);
+}
+
+HIPATTN_EXPORT hipattn_status hipattn_paged_attention_i8(const hipattn_pa_desc* desc, const void* q, const void* k_new, const void* v_new,
+                                                         void* key_cache, void* value_cache, float* key_scales, float* value_scales,
+                                                         const int32_t* past_lens, const int32_t* subsequence_begins,
+                                                         const int32_t* block_indices, const int32_t* block_indices_begins, void* out,
+                                                         void* workspace, size_t workspace_bytes, hipattn_stream stream) {
+    if (desc && desc->cache_dtype != HIPATTN_I8) return fail(HIPATTN_INVALID_ARGUMENT, "paged_attention_i8: cache dtype %d", desc->cache_dtype);
+    return paged_attention_impl(desc, q, k_new, v_new, key_cache, value_cache, past_lens, subsequence_begins, block_indices,
+                                block_indices_begins, out, workspace, workspace_bytes, stream, false, key_scales, value_scales);
 }
 
 HIPATTN_EXPORT hipattn_status hipattn_paged_attention_noalloc(const hipattn_pa_desc* desc, const void* q,
@@ -621,6 +738,7 @@ HIPATTN_EXPORT hipattn_status hipattn_paged_attention_scores(const hipattn_pa_de
     if (!q || !key_cache || !past_lens || !subsequence_begins || !block_indices || !block_indices_begins || !scores)
         return fail(HIPATTN_INVALID_ARGUMENT, "paged_attention_scores: null pointer");
     if (desc->num_seqs > 65535) return fail(HIPATTN_UNSUPPORTED, "paged_attention_scores: %d sequences (at most 65535)", desc->num_seqs);
+    if (desc->cache_dtype == HIPATTN_I8) return fail(HIPATTN_UNSUPPORTED, "paged_attention_scores: no scores from i8 caches");
     if (desc->alibi_slopes) return fail(HIPATTN_UNSUPPORTED, "paged_attention_scores: no distance bias (alibi_slopes) in the scores kernels");
     if (desc->sinks) return fail(HIPATTN_UNSUPPORTED, "paged_attention_scores: no attention sinks in the scores kernels");
     const size_t need = (size_t)desc->num_tokens * desc->num_heads_q * sizeof(float);

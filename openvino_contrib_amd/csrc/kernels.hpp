@@ -56,6 +56,44 @@ struct KeyRotationParams {
 };
 hipError_t launch_rotate_key_cache(const KeyRotationParams& p, hipStream_t stream);
 
+// New keys and values into the caches, rotated on the way, and the queries rotated beside them (rope_append.hip).  Strides in
+// elements, resolved (none is 0 for lack of a value).
+struct RopeAppendParams {
+    const void* q;  // nullptr: append alone
+    const void* k_new;
+    const void* v_new;
+    const void* cos;  // nullptr: no rotation
+    const void* sin;
+    const int32_t* positions;  // nullptr: the tokens' cache positions
+    void* q_out;
+    uint8_t* key_cache;
+    uint8_t* value_cache;
+    float* key_scales;  // HIPATTN_I8 only
+    float* value_scales;
+    const int32_t* past_lens;
+    const int32_t* subsequence_begins;
+    const int32_t* block_indices;
+    const int32_t* block_indices_begins;
+    int64_t q_token, k_token, v_token, out_token;
+    int64_t q_head, k_head, v_head, out_head;
+    int64_t table_row_stride;
+    int table_rows;
+    int table_dtype;
+    int rotary;
+    int interleaved;
+    int q_dtype;
+    int kv_dtype;
+    int cache_dtype;
+    int num_heads_q;
+    int num_heads_kv;
+    int head_dim;
+    int block_size;
+    int num_blocks;
+    int num_tokens;
+    int num_seqs;
+};
+hipError_t launch_rope_append(const RopeAppendParams& p, hipStream_t stream);
+
 // Wavefronts the writer needs for p (and p.heads_per_wave, which it sets).
 inline int64_t kv_write_wavefronts(KvWriteParams& p) {
     const auto aligned16 = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
@@ -97,6 +135,8 @@ struct PagedParams {
     const void* q;
     const uint8_t* key_cache;
     const uint8_t* value_cache;
+    const float* key_scales;    // HIPATTN_I8: [num_blocks, the cache's kv heads]
+    const float* value_scales;
     const int32_t* past_lens;
     const int32_t* subsequence_begins;
     const int32_t* block_indices;
