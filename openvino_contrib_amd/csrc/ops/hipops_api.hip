@@ -117,3 +117,20 @@ HIPOPS_API hipattn_status hipops_glu(const void* x, void* out, int64_t rows, int
                                      int dtype, hipattn_stream stream) {
     return guarded("hipops_glu", [&] { return glu(x, out, rows, width, activation, gate_first, dtype, (hipStream_t)stream); });
 }
+
+HIPOPS_API hipattn_status hipops_quantize_rows(const hipops_quantize_desc* desc, const void* x, const void* gamma, int8_t* codes, float* scales,
+                                               hipattn_stream stream) {
+    return guarded("hipops_quantize_rows", [&] { return quantize_rows(desc, x, gamma, codes, scales, (hipStream_t)stream); });
+}
+
+HIPOPS_API hipattn_status hipops_matmul_i8_workspace_size(const hipops_matmul_i8_desc* desc, size_t* bytes) {
+    return guarded("hipops_matmul_i8_workspace_size", [&] { return matmul_i8_workspace_size(desc, bytes); });
+}
+
+HIPOPS_API hipattn_status hipops_matmul_i8(const hipops_matmul_i8_desc* desc, const int8_t* a, const float* a_scales, const int8_t* b,
+                                           const float* b_scales, const void* bias, const void* residual, void* c, void* workspace,
+                                           size_t workspace_bytes, hipattn_stream stream) {
+    return guarded("hipops_matmul_i8", [&] {
+        return matmul_i8(desc, a, a_scales, b, b_scales, bias, residual, c, workspace, workspace_bytes, (hipStream_t)stream);
+    });
+}

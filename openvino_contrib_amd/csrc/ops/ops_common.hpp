@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "hipops.h"
+#include "hipops_int8.h"
 #include "ops/projection.h"
 
 namespace hipops {
@@ -41,6 +42,10 @@ hipattn_status projection(const hipops_projection_desc* desc, const hipops_proje
                           hipStream_t stream);
 hipattn_status residual_norm(const void* product, const void* residual, const void* gamma, void* out, void* normalised, int64_t rows, int64_t n,
                              float eps, int dtype, int gamma_dtype, hipStream_t stream);
+hipattn_status quantize_rows(const hipops_quantize_desc* desc, const void* x, const void* gamma, int8_t* codes, float* scales, hipStream_t stream);
+hipattn_status matmul_i8_workspace_size(const hipops_matmul_i8_desc* desc, size_t* bytes);
+hipattn_status matmul_i8(const hipops_matmul_i8_desc* desc, const int8_t* a, const float* a_scales, const int8_t* b, const float* b_scales,
+                         const void* bias, const void* residual, void* c, void* workspace, size_t workspace_bytes, hipStream_t stream);
 hipattn_status matmul_workspace_size(const hipops_matmul_desc* desc, size_t* bytes);
 hipattn_status matmul(const hipops_matmul_desc* desc, const void* a, const void* b, void* c, void* workspace,
                       size_t workspace_bytes, hipStream_t stream);

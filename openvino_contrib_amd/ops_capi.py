@@ -1,5 +1,5 @@
-"""ctypes binding of libhipops.so (include/hipops.h): RMS norm, RoPE, MatMul, Gather, Concat, Swish,
-Multiply, GLU, Transpose, Convert, broadcasting arithmetic, Softmax.
+"""ctypes binding of libhipops.so (include/hipops.h, include/hipops_int8.h): RMS norm, RoPE, MatMul, Gather, Concat, Swish,
+Multiply, GLU, Transpose, Convert, broadcasting arithmetic, Softmax, products of 8-bit codes.
 
 Device memory, streams and events come from the hipattn binding (capi.DeviceBuffer & co.); this
 module adds the operator calls.  No fallback: a missing library or a failed call raises.
@@ -62,6 +62,15 @@ class ProjectionArgs(ctypes.Structure):
                 ("normalised", _vp)]
 
 
+class QuantizeDesc(ctypes.Structure):
+    _fields_ = [("source", _i), ("x_dtype", _i), ("gamma_dtype", _i), ("glu_activation", _i), ("glu_gate_first", _i), ("eps", _f), ("rows", _i64),
+                ("width", _i64), ("x_row_stride", _i64)]
+
+
+class MatmulI8Desc(ctypes.Structure):
+    _fields_ = [("c_dtype", _i), ("m", _i64), ("n", _i64), ("k", _i64), ("lda", _i64), ("ldb", _i64), ("ldc", _i64)]
+
+
 PROJECTION_ROPE, PROJECTION_ADD, PROJECTION_GLU = 0, 1, 2
 
 SYMBOLS = {
@@ -82,6 +91,13 @@ SYMBOLS = {
     "hipops_concat": (_i, [_P(_vp), _P(_i64), _i, _i64, _vp, _vp]),
 }
 
+# include/hipops_int8.h
+SYMBOLS_INT8 = {
+    "hipops_quantize_rows": (_i, [_P(QuantizeDesc), _vp, _vp, _vp, _vp, _vp]),
+    "hipops_matmul_i8_workspace_size": (_i, [_P(MatmulI8Desc), _P(_sz)]),
+    "hipops_matmul_i8": (_i, [_P(MatmulI8Desc)] + [_vp] * 8 + [_sz, _vp]),
+}
+
 _lib = None
 
 
@@ -99,7 +115,7 @@ def lib():
             raise HipOpsError(-1, "%s is missing: run __graft_entry__.build() or "
                                   "python -m openvino_contrib_amd.build" % LIB_PATH)
         L = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in SYMBOLS.items():
+        for name, (res, args) in {**SYMBOLS, **SYMBOLS_INT8}.items():
             fn = getattr(L, name)  # AttributeError if the symbol is not exported
             fn.restype = res
             fn.argtypes = args
@@ -208,3 +224,23 @@ def concat(inputs, axis_bytes, outer, out, stream=None):
     ptrs = (_vp * n)(*[b.ptr.value if b is not None else None for b in inputs])
     widths = (_i64 * n)(*axis_bytes)
     check(lib().hipops_concat(ptrs, widths, n, outer, _ptr(out), _h(stream)))
+
+
+QUANTIZE_PLAIN, QUANTIZE_RMS_NORM, QUANTIZE_GLU = 0, 1, 2
+
+
+def quantize_rows(desc, x, gamma, codes, scales, stream=None):
+    """Rows of x, of its RMS norm (gamma may be None) or of its GLU as 8-bit codes with a scale each."""
+    check(lib().hipops_quantize_rows(ctypes.byref(desc), _ptr(x), _ptr(gamma), _ptr(codes), _ptr(scales), _h(stream)))
+
+
+def matmul_i8_workspace_size(desc):
+    n = _sz(0)
+    check(lib().hipops_matmul_i8_workspace_size(ctypes.byref(desc), ctypes.byref(n)))
+    return n.value
+
+
+def matmul_i8(desc, a, a_scales, b, b_scales, bias, residual, c, workspace=None, stream=None):
+    """c = a_scales b_scales (a b^T) + bias + residual; scales, bias and residual may be None."""
+    check(lib().hipops_matmul_i8(ctypes.byref(desc), *[_ptr(x) for x in (a, a_scales, b, b_scales, bias, residual, c, workspace)],
+                                 workspace.nbytes if workspace is not None else 0, _h(stream)))
