@@ -117,6 +117,9 @@ __host__ __device__ __forceinline__ int64_t cache_row_bytes(int cache_dtype, int
     }
 }
 
+// caches of one byte per element
+__host__ __device__ __forceinline__ bool eight_bit(int cache_dtype) { return cache_dtype == HIPATTN_U8 || cache_dtype == HIPATTN_I8; }
+
 // one element of a cache row, dequantised (i8: the code; its scale is the block's)
 __device__ __forceinline__ float load_cache_elem(const uint8_t* row, int d, int cache_dtype) {
     switch (cache_dtype) {
@@ -164,6 +167,27 @@ __device__ __forceinline__ uint4_t dequant8(uint2_t w, half2_t scale, half2_t of
     r[1] = __builtin_bit_cast(uint32_t, (biased_half2(w[0], 0x04030402u) - bias) * scale + off);
     r[2] = __builtin_bit_cast(uint32_t, (biased_half2(w[1], 0x04010400u) - bias) * scale + off);
     r[3] = __builtin_bit_cast(uint32_t, (biased_half2(w[1], 0x04030402u) - bias) * scale + off);
+    return r;
+}
+
+// 8 signed codes -> 8 fp16 values code * scale.  The scale goes in as two fp16 numbers, its rounded value and what that left over:
+// rounded to one, it would be off by the same 2^-12 for every key of a block, which scores of some tens do not average out.
+struct SplitScale {
+    half2_t high, low;
+};
+__device__ __forceinline__ SplitScale split_scale(float scale) {
+    const half_t high = (half_t)scale, low = (half_t)(scale - (float)high);
+    return {half2_t{high, high}, half2_t{low, low}};
+}
+__device__ __forceinline__ uint4_t dequant_codes8(uint2_t w, const SplitScale& s) {
+    const half2_t bias = {(half_t)1152.0f, (half_t)1152.0f};  // (the sign bit flipped: 1024 + 128 + code)
+    const uint2_t b = w ^ 0x80808080u;
+    uint4_t r;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const half2_t c = biased_half2(b[i >> 1], (i & 1) ? 0x04030402u : 0x04010400u) - bias;
+        r[i] = __builtin_bit_cast(uint32_t, c * s.high + c * s.low);
+    }
     return r;
 }
 

@@ -131,6 +131,9 @@ struct Tile {
     int64_t block_stride;   // paged: bytes between physical blocks
     int block_size;
     int block_shift;        // log2(block_size)
+    const float* k_scales;  // i8 caches: the scales of this kv head, scale_stride from block to block
+    const float* v_scales;
+    int scale_stride;
     // dense SDPA with an attention mask (kMask variants of the kernel): the mask element of the
     // tile's query row 0 and key 0 for this batch and head; rows mask_row_bytes apart (0: one row
     // for every query), keys side by side
@@ -142,6 +145,7 @@ struct Tile {
 // of the kernel loads them into registers, dequantises to fp16 and writes the result into the
 // same LDS stages (same layout) the 16-bit caches are loaded into directly; everything behind
 // that is the fp16 kernel.
+// i8 caches (kI8) are the same with rows of 128 payload bytes and the scale of their block.
 constexpr int kU8RowBytes = kD + 8;
 struct U8Rows {
     uint2_t k_lo, k_hi, v_lo, v_hi;  // this lane's 16 payload bytes of a K row and of a V row
@@ -615,7 +619,7 @@ __device__ __forceinline__ void barrier_keeping_loads(int keep) {  // keep is ev
 // chunk of a row does not exist fetches the row's first chunk instead -- valid, finite data that only
 // ever meets the zeros the query fragments hold in those columns, or lands in output columns that
 // are not stored.
-template <bool kBf16, bool kU8 = false, bool kPaged = true, int kMask = 0, bool kPad = false>
+template <bool kBf16, bool kU8 = false, bool kPaged = true, int kMask = 0, bool kPad = false, bool kI8 = false>
 __device__ __forceinline__ void run_pair(const Tile& t, int kv_lo, int kv_hi, uint8_t* lds_generic, float scale) {
     static_assert(kPaged || !kU8, "dense K/V are 16-bit");
     static_assert(!kPad || !kU8, "smaller head sizes: 16-bit K/V");
@@ -623,6 +627,7 @@ __device__ __forceinline__ void run_pair(const Tile& t, int kv_lo, int kv_hi, ui
     const int head_chunks = kPad ? t.head_dim >> 3 : kD / 8;
     static_assert(kMask == 0 || !kPaged, "attention masks belong to the dense operator");
     static_assert(!(kU8 && kBf16), "u8 caches are dequantised to fp16");
+    static_assert(!kI8 || kU8, "i8 caches run the 8-bit form");
     using M = Mfma<kBf16>;
     using vec8 = typename M::vec8;
     lds_byte* const lds = (lds_byte*)lds_generic;
@@ -808,7 +813,10 @@ __device__ __forceinline__ void run_pair(const Tile& t, int kv_lo, int kv_hi, ui
     // ---- u8 caches: lane l of wavefront w handles 16 payload bytes (piece l % 8) of row 8w + l / 8
     const int u8_row = 8 * wave + (lane >> 3), u8_piece = lane & 7;
     // address of this lane's row of tile j (entry: the block table entry of the wavefront's rows)
-    auto u8_row_address = [&](const uint8_t* base, int j, int entry) __attribute__((always_inline)) -> const uint8_t* {
+    constexpr int kByteRow = kI8 ? kD : kU8RowBytes;
+    // (and kI8: the block's scale.  What a block outside the cache, or one that no key of the tile is attended in, may hold
+    // beside codes that are never used -- infinities, NaN -- becomes zero, as its probabilities would not make it that.)
+    auto u8_row_address = [&](const uint8_t* base, int j, int entry, const float* scales, float& scale) __attribute__((always_inline)) -> const uint8_t* {
         const int key0 = kv_lo + j * kTileK + 8 * wave;
         int key = kv_lo + j * kTileK + u8_row;
         int pb;
@@ -818,8 +826,12 @@ __device__ __forceinline__ void run_pair(const Tile& t, int kv_lo, int kv_hi, ui
             key = min(key, t.kv_len - 1);
             pb = t.table[key >> t.block_shift];
         }
-        pb = min(max(pb, 0), t.num_blocks - 1);
-        return base + (int64_t)pb * t.block_stride + (int64_t)(key & (t.block_size - 1)) * kU8RowBytes;
+        const int inside = min(max(pb, 0), t.num_blocks - 1);
+        if constexpr (kI8) {
+            scale = scales[(int64_t)inside * t.scale_stride];
+            scale = inside == pb && fabsf(scale) < INFINITY ? scale : 0.0f;
+        }
+        return base + (int64_t)inside * t.block_stride + (int64_t)(key & (t.block_size - 1)) * kByteRow;
     };
     auto u8_fetch = [&](int jk, int ek, int jv, int ev) __attribute__((always_inline)) -> U8Rows {
         U8Rows x;
@@ -828,16 +840,28 @@ __device__ __forceinline__ void run_pair(const Tile& t, int kv_lo, int kv_hi, ui
         x.jk = jk < n ? jk : -1;
         x.jv = jv < n ? jv : -1;
         if (x.jk >= 0) {
-            const uint8_t* row = u8_row_address(t.k, jk, ek);
-            x.k_sz = *(const float2*)row;
-            x.k_lo = *(const uint2_t*)(row + 8 + 16 * u8_piece);
-            x.k_hi = *(const uint2_t*)(row + 16 + 16 * u8_piece);
+            const uint8_t* row = u8_row_address(t.k, jk, ek, t.k_scales, x.k_sz.x);
+            if constexpr (kI8) {
+                const uint4_t w = *(const uint4_t*)(row + 16 * u8_piece);
+                x.k_lo = (uint2_t){w[0], w[1]};
+                x.k_hi = (uint2_t){w[2], w[3]};
+            } else {
+                x.k_sz = *(const float2*)row;
+                x.k_lo = *(const uint2_t*)(row + 8 + 16 * u8_piece);
+                x.k_hi = *(const uint2_t*)(row + 16 + 16 * u8_piece);
+            }
         }
         if (x.jv >= 0) {
-            const uint8_t* row = u8_row_address(t.v, jv, ev);
-            x.v_sz = *(const float2*)row;
-            x.v_lo = *(const uint2_t*)(row + 8 + 16 * u8_piece);
-            x.v_hi = *(const uint2_t*)(row + 16 + 16 * u8_piece);
+            const uint8_t* row = u8_row_address(t.v, jv, ev, t.v_scales, x.v_sz.x);
+            if constexpr (kI8) {
+                const uint4_t w = *(const uint4_t*)(row + 16 * u8_piece);
+                x.v_lo = (uint2_t){w[0], w[1]};
+                x.v_hi = (uint2_t){w[2], w[3]};
+            } else {
+                x.v_sz = *(const float2*)row;
+                x.v_lo = *(const uint2_t*)(row + 8 + 16 * u8_piece);
+                x.v_hi = *(const uint2_t*)(row + 16 + 16 * u8_piece);
+            }
         }
         return x;
     };
@@ -846,20 +870,36 @@ __device__ __forceinline__ void run_pair(const Tile& t, int kv_lo, int kv_hi, ui
     auto u8_store = [&](const U8Rows& x) __attribute__((always_inline)) {
         typedef __attribute__((address_space(3))) uint4_t lds_uint4;
         if (x.jk >= 0) {
-            const half2_t sc = {(half_t)x.k_sz.x, (half_t)x.k_sz.x};
-            const float o32 = -x.k_sz.y * x.k_sz.x;
-            const half2_t of = {(half_t)o32, (half_t)o32};
             lds_byte* const rowp = k_stage(x.jk) + u8_row * kRowBytes;
-            *(lds_uint4*)(rowp + (((2 * u8_piece) ^ (u8_row & 15)) << 4)) = dequant8(x.k_lo, sc, of);
-            *(lds_uint4*)(rowp + (((2 * u8_piece + 1) ^ (u8_row & 15)) << 4)) = dequant8(x.k_hi, sc, of);
+            lds_uint4* const lo = (lds_uint4*)(rowp + (((2 * u8_piece) ^ (u8_row & 15)) << 4));
+            lds_uint4* const hi8 = (lds_uint4*)(rowp + (((2 * u8_piece + 1) ^ (u8_row & 15)) << 4));
+            if constexpr (kI8) {  // (softmax scale and log2(e) on the keys instead of the queries: one rounding of the product less)
+                const SplitScale sc = split_scale(x.k_sz.x * c);
+                *lo = dequant_codes8(x.k_lo, sc);
+                *hi8 = dequant_codes8(x.k_hi, sc);
+            } else {
+                const half2_t sc = {(half_t)x.k_sz.x, (half_t)x.k_sz.x};
+                const float o32 = -x.k_sz.y * x.k_sz.x;
+                const half2_t of = {(half_t)o32, (half_t)o32};
+                *lo = dequant8(x.k_lo, sc, of);
+                *hi8 = dequant8(x.k_hi, sc, of);
+            }
         }
         if (x.jv >= 0) {
-            const half2_t sc = {(half_t)x.v_sz.x, (half_t)x.v_sz.x};
-            const float o32 = -x.v_sz.y * x.v_sz.x;
-            const half2_t of = {(half_t)o32, (half_t)o32};
             lds_byte* const rowp = v_stage(x.jv) + u8_row * kRowBytes;
-            *(lds_uint4*)(rowp + (((2 * u8_piece) ^ (4 * (u8_row & 3))) << 4)) = dequant8(x.v_lo, sc, of);
-            *(lds_uint4*)(rowp + (((2 * u8_piece + 1) ^ (4 * (u8_row & 3))) << 4)) = dequant8(x.v_hi, sc, of);
+            lds_uint4* const lo = (lds_uint4*)(rowp + (((2 * u8_piece) ^ (4 * (u8_row & 3))) << 4));
+            lds_uint4* const hi8 = (lds_uint4*)(rowp + (((2 * u8_piece + 1) ^ (4 * (u8_row & 3))) << 4));
+            if constexpr (kI8) {
+                const SplitScale sc = split_scale(x.v_sz.x);
+                *lo = dequant_codes8(x.v_lo, sc);
+                *hi8 = dequant_codes8(x.v_hi, sc);
+            } else {
+                const half2_t sc = {(half_t)x.v_sz.x, (half_t)x.v_sz.x};
+                const float o32 = -x.v_sz.y * x.v_sz.x;
+                const half2_t of = {(half_t)o32, (half_t)o32};
+                *lo = dequant8(x.v_lo, sc, of);
+                *hi8 = dequant8(x.v_hi, sc, of);
+            }
         }
     };
     // the workgroup barrier of the u8 variant: LDS writes done, register loads may stay in flight
@@ -918,6 +958,7 @@ __device__ __forceinline__ void run_pair(const Tile& t, int kv_lo, int kv_hi, ui
     else
         wait_keeping_loads(first + recent);
     // Q^T operand: k-step i covers head-dim i*16 + hi*8 .. +8
+    const float q_factor = kI8 ? 1.0f : c;
     vec8 qf[8];
     {
         typedef __attribute__((address_space(3))) uint4_t lds_uint4;
@@ -929,10 +970,10 @@ __device__ __forceinline__ void run_pair(const Tile& t, int kv_lo, int kv_hi, ui
         }
         if (t.q_dtype == HIPATTN_BF16) {  // (one wave-uniform branch, not a choice per element)
 #pragma unroll
-            for (int i = 0; i < 8; i++) qf[i] = convert_q_frag<kBf16, true>(raw[i], c);
+            for (int i = 0; i < 8; i++) qf[i] = convert_q_frag<kBf16, true>(raw[i], q_factor);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) qf[i] = convert_q_frag<kBf16, false>(raw[i], c);
+            for (int i = 0; i < 8; i++) qf[i] = convert_q_frag<kBf16, false>(raw[i], q_factor);
         }
     }
 #pragma unroll
@@ -1134,7 +1175,7 @@ __device__ __forceinline__ int small_div(int a, int b) {
     q -= (r < 0) ? 1 : 0;
     return q;
 }
-template <bool kBf16, bool kU8 = false, bool kPaged = true, int kMask = 0, bool kPad = false>
+template <bool kBf16, bool kU8 = false, bool kPaged = true, int kMask = 0, bool kPad = false, bool kI8 = false>
 __device__ __forceinline__ void run_both(const Tile& t0, const Tile& t1, uint8_t* lds, float scale) {
     int lo0, hi0, lo1, hi1;
     key_range(t0, lo0, hi0);
@@ -1151,7 +1192,7 @@ __device__ __forceinline__ void run_both(const Tile& t0, const Tile& t1, uint8_t
         kv_hi = max(hi0, hi1);
     }
     const int group = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8);
-    run_pair<kBf16, kU8, kPaged, kMask, kPad>(group ? t1 : t0, kv_lo, kv_hi, lds, scale);
+    run_pair<kBf16, kU8, kPaged, kMask, kPad, kI8>(group ? t1 : t0, kv_lo, kv_hi, lds, scale);
 }
 
 // One workgroup per (128-row query tile of a multi-token sequence, pair of query heads) or, with an
@@ -1179,7 +1220,7 @@ __device__ __forceinline__ Tile paged_group_tile(const PagedParams& p, int s, in
     t.q_dtype = p.q_dtype;
     t.out_dtype = p.out_dtype;
     t.head_dim = D;
-    const int row_bytes = p.cache_dtype == HIPATTN_U8 ? kU8RowBytes : D * 2;
+    const int row_bytes = p.cache_dtype == HIPATTN_U8 ? kU8RowBytes : p.cache_dtype == HIPATTN_I8 ? D : D * 2;
     const int64_t head_off = (int64_t)(h / G) * p.block_size * row_bytes;
     t.k = p.key_cache + head_off;
     t.v = p.value_cache + head_off;
@@ -1189,6 +1230,11 @@ __device__ __forceinline__ Tile paged_group_tile(const PagedParams& p, int s, in
     t.block_stride = (int64_t)p.num_heads_kv * p.block_size * row_bytes;
     t.block_size = p.block_size;
     t.block_shift = __builtin_ctz(p.block_size);
+    if (p.cache_dtype == HIPATTN_I8) {
+        t.k_scales = p.key_scales + h / G;
+        t.v_scales = p.value_scales + h / G;
+        t.scale_stride = p.num_heads_kv;
+    }
     t.mask = nullptr;
     t.mask_row_bytes = 0;
     return t;
@@ -1196,7 +1242,7 @@ __device__ __forceinline__ Tile paged_group_tile(const PagedParams& p, int s, in
 
 // kPad: a head size between 64 and 128 (p.head_dim, a multiple of 8; 16-bit caches).
 // kShadow: sequences that begin with this call take their rows from the prologue's dequantised copy (p.shadow_table), where there is one.
-template <bool kBf16, bool kU8, bool kPad, bool kShadow = false>
+template <bool kBf16, bool kU8, bool kPad, bool kShadow = false, bool kI8 = false>
 __device__ __forceinline__ void paged_prefill_item(const PagedParams& p, int index, uint8_t* lds) {
     // Launch index (a workgroup's number on the device modulo 8) -> work item.  The workgroups that run on one XCD at a time should share K/V in
     // its L2, and the XCDs should get equal work although sequences differ in length.  With a
@@ -1256,7 +1302,7 @@ __device__ __forceinline__ void paged_prefill_item(const PagedParams& p, int ind
             return;
         }
     }
-    run_both<kBf16, kU8, true, 0, kPad>(t0, t1, lds, p.scale);
+    run_both<kBf16, kU8, true, 0, kPad, kI8>(t0, t1, lds, p.scale);
 }
 
 }  // namespace flash

@@ -94,10 +94,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     run_both<kBf16, false, false, kMask, true>(t0, t1, lds, p.scale);
 }
 
-template <bool kBf16, bool kU8>
+template <bool kBf16, bool kU8, bool kI8 = false>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_prefill_kernel(PagedParams p) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kLdsBytes];
-    paged_prefill_item<kBf16, kU8, false>(p, (int)blockIdx.x, lds);
+    paged_prefill_item<kBf16, kU8, false, false, kI8>(p, (int)blockIdx.x, lds);
 }
 
 // The same for a head size between 64 and 128 (16-bit caches): the kPad form of the loop.
@@ -187,7 +187,7 @@ hipError_t launch_sdpa_flash(const SdpaParams& p, hipStream_t stream, const Kern
 
 hipError_t launch_paged_prefill(const PagedParams& p, hipStream_t stream) {
     // the head sizes between 64 and 128 of a 16-bit cache: this kernel on rows of fewer columns
-    const bool padded = p.head_dim > 64 && p.head_dim < flash::kD && p.head_dim % 8 == 0 && p.cache_dtype != HIPATTN_U8 &&
+    const bool padded = p.head_dim > 64 && p.head_dim < flash::kD && p.head_dim % 8 == 0 && !eight_bit(p.cache_dtype) &&
                         (((uintptr_t)p.q | (uintptr_t)p.key_cache | (uintptr_t)p.value_cache | (uintptr_t)p.out) & 15) == 0;
     // (ALiBi, attention sinks: the plain kernel has the distance term and the sink in its denominator; the tuned one
     // has no vector slot to spare for the one and was not given the other)
@@ -201,6 +201,8 @@ hipError_t launch_paged_prefill(const PagedParams& p, hipStream_t stream) {
             hipLaunchKernelGGL(flash::paged_prefill_padded_kernel<false>, grid, dim3(flash::kThreads), 0, stream, p);
     } else if (p.cache_dtype == HIPATTN_BF16)
         hipLaunchKernelGGL((flash::paged_prefill_kernel<true, false>), grid, dim3(flash::kThreads), 0, stream, p);
+    else if (p.cache_dtype == HIPATTN_I8)
+        hipLaunchKernelGGL((flash::paged_prefill_kernel<false, true, true>), grid, dim3(flash::kThreads), 0, stream, p);
     else if (p.cache_dtype == HIPATTN_U8)
         hipLaunchKernelGGL((flash::paged_prefill_kernel<false, true>), grid, dim3(flash::kThreads), 0, stream, p);
     else

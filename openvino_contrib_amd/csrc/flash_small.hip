@@ -178,6 +178,9 @@ struct Work {
     int block_shift;        // log2(block size)
     int num_blocks;
     int64_t block_stride;   // bytes from one cache block to the next
+    const float* k_scales;  // i8 caches: the scales of this kv head, scale_stride from block to block
+    const float* v_scales;
+    int scale_stride;
     float scale;
     const float* alibi;     // paged: nullptr, or the ALiBi slope of row 0's query head; row r's is alibi[r * alibi_step]
     int alibi_step;         // 0: every row belongs to one head; 1: the rows are consecutive query heads
@@ -197,8 +200,10 @@ __device__ __forceinline__ uint32_t pack2(int dtype, float lo, float hi) {
 // kU8 (paged, fp16 products): the cache rows are [scale f32][zero-point f32][head_dim bytes]; a piece
 // travels as its eight bytes and the row's scale and zero-point and becomes eight fp16 values
 // (byte - zero-point) * scale on its way into LDS.
-template <bool kBf16, bool kMask, bool kPaged, int kDP, bool kU8 = false, int kUsed = kDP>
+// kI8: rows of head_dim codes, which travel with the scale of their block.
+template <bool kBf16, bool kMask, bool kPaged, int kDP, bool kU8 = false, int kUsed = kDP, bool kI8 = false>
 __device__ __forceinline__ void attend(const Work& w, uint8_t (*lds)[2][tile_bytes<kDP>()]) {
+    static_assert(!kI8 || kU8, "i8 caches run the 8-bit form");
     static_assert(!kU8 || (kPaged && !kBf16), "u8 rows exist in paged caches and are multiplied as fp16");
     // kUsed: the columns the products run over (w.head_dim <= kUsed <= kDP, a multiple of 16); the rows in LDS
     // keep the layout of kDP columns
@@ -208,7 +213,8 @@ __device__ __forceinline__ void attend(const Work& w, uint8_t (*lds)[2][tile_byt
     using vec8 = typename M::vec8;
     constexpr int kChunks = kDP / 8;             // 16-byte chunks of a row in LDS
     const int chunks = w.head_dim >> 3;          // ... of which the call's rows fill this many
-    const int row_bytes = kU8 ? w.head_dim + 8 : w.head_dim * 2;
+    constexpr int kRowHead = kI8 ? 0 : 8;  // (8-bit rows) bytes ahead of the payload
+    const int row_bytes = kU8 ? w.head_dim + kRowHead : w.head_dim * 2;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int n32 = lane & 31, hi = lane >> 5;
     const int my_row = wave * 32 + n32;          // this lane's query row in the tile (may lie beyond w.rows)
@@ -277,17 +283,28 @@ __device__ __forceinline__ void attend(const Work& w, uint8_t (*lds)[2][tile_byt
             const int piece = tid + 64 * kWaves * s, r = piece / kChunks, c = piece % kChunks;
             const int key = min(tile * kTileK + r, w.kv_len - 1);  // rows past the end repeat the last key (masked later)
             int64_t at;
+            float k_scale = 0.0f, v_scale = 0.0f;
             if constexpr (kPaged) {
                 // a block id outside the cache is redirected into it, and its keys are masked
                 const int pb = min(max(block_of[s], 0), w.num_blocks - 1);
                 if (pb != block_of[s]) bad |= 1u << s;
+                if constexpr (kI8) {  // (a block with nothing attended may have any scale beside codes that do not count)
+                    k_scale = w.k_scales[(int64_t)pb * w.scale_stride];
+                    v_scale = w.v_scales[(int64_t)pb * w.scale_stride];
+                    k_scale = pb == block_of[s] && fabsf(k_scale) < INFINITY ? k_scale : 0.0f;
+                    v_scale = pb == block_of[s] && fabsf(v_scale) < INFINITY ? v_scale : 0.0f;
+                }
                 at = (int64_t)pb * w.block_stride + (int64_t)(key & ((1 << w.block_shift) - 1)) * row_bytes + (kU8 ? 0 : 16 * c);
             } else {
                 at = (int64_t)key * row_bytes + 16 * c;
             }
             stage[s] = stage[kPieces + s] = (uint4_t){0u, 0u, 0u, 0u};
             if (c < chunks) {
-                if constexpr (kU8) {
+                if constexpr (kI8) {
+                    const uint2_t kraw = *(const uint2_t*)(w.k + at + 8 * c), vraw = *(const uint2_t*)(w.v + at + 8 * c);
+                    stage[s] = (uint4_t){kraw[0], kraw[1], __float_as_uint(k_scale), 0u};
+                    stage[kPieces + s] = (uint4_t){vraw[0], vraw[1], __float_as_uint(v_scale), 0u};
+                } else if constexpr (kU8) {
                     const uint2_t kraw = *(const uint2_t*)(w.k + at + 8 + 8 * c), ksz = *(const uint2_t*)(w.k + at);
                     const uint2_t vraw = *(const uint2_t*)(w.v + at + 8 + 8 * c), vsz = *(const uint2_t*)(w.v + at);
                     stage[s] = (uint4_t){kraw[0], kraw[1], ksz[0], ksz[1]};
@@ -306,7 +323,11 @@ __device__ __forceinline__ void attend(const Work& w, uint8_t (*lds)[2][tile_byt
             if constexpr (kPaged) {
                 if (c == 0) row_bad[buf][r] = (uint8_t)((bad >> s) & 1u);
             }
-            if constexpr (kU8) {
+            if constexpr (kI8) {
+                const auto values = [](const uint4_t& x) { return dequant_codes8((uint2_t){x[0], x[1]}, split_scale(__uint_as_float(x[2]))); };
+                *(uint4_t*)(lds[buf][0] + k_chunk_offset<kDP>(r, c)) = values(stage[s]);
+                *(uint4_t*)(lds[buf][1] + v_chunk_offset<kDP>(r, c)) = values(stage[kPieces + s]);
+            } else if constexpr (kU8) {
                 *(uint4_t*)(lds[buf][0] + k_chunk_offset<kDP>(r, c)) = dequantised8(stage[s]);
                 *(uint4_t*)(lds[buf][1] + v_chunk_offset<kDP>(r, c)) = dequantised8(stage[kPieces + s]);
             } else {
@@ -586,7 +607,7 @@ __global__ __launch_bounds__(64 * kWaves) void sdpa_flash_small_masked_kernel(Sd
 // p.tile_prefix (written on the device by the plan of the decode path or by paged_tiles_plan_kernel),
 // the later -- heavier -- tiles of a sequence first.  One workgroup per (tile, head); the grid is
 // an upper bound.
-template <bool kBf16, int kDP, bool kU8 = false, int kUsed = kDP>
+template <bool kBf16, int kDP, bool kU8 = false, int kUsed = kDP, bool kI8 = false>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))) void paged_tiles_kernel(PagedParams p) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][tile_bytes<kDP>()];
     const int item = blockIdx.x / p.num_heads_q, h = blockIdx.x % p.num_heads_q;
@@ -627,7 +648,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     w.causal = 1;
     w.window = p.sliding_window;
     w.kv_len = min(past + qlen, table_len * p.block_size);
-    const int row_bytes = kU8 ? D + 8 : D * 2;
+    const int row_bytes = kI8 ? D : kU8 ? D + 8 : D * 2;
     const int64_t head_off = (int64_t)hkv * p.block_size * row_bytes;
     w.k = p.key_cache + head_off;
     w.v = p.value_cache + head_off;
@@ -635,6 +656,11 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     w.block_shift = __builtin_ctz(p.block_size);
     w.num_blocks = p.num_blocks;
     w.block_stride = (int64_t)p.num_heads_kv * p.block_size * row_bytes;
+    if constexpr (kI8) {
+        w.k_scales = p.key_scales + hkv;
+        w.v_scales = p.value_scales + hkv;
+        w.scale_stride = p.num_heads_kv;
+    }
     w.scale = p.scale;
     w.alibi = p.alibi_slopes ? p.alibi_slopes + (heads_as_rows ? h * G : h) : nullptr;
     w.alibi_step = heads_as_rows ? 1 : 0;
@@ -642,7 +668,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     w.mask = nullptr;
     w.mask_row_stride = w.mask_key_stride = 0;
     w.mask_dtype = 0;
-    attend<kBf16, false, true, kDP, kU8, kUsed>(w, lds);
+    attend<kBf16, false, true, kDP, kU8, kUsed, kI8>(w, lds);
 }
 
 // tile_prefix for a batch in which every sequence with tokens goes through paged_tiles_kernel
@@ -728,7 +754,16 @@ hipError_t launch_sdpa_flash_small(const SdpaParams& p, hipStream_t stream, cons
 static void launch_tiles(const PagedParams& p, unsigned groups, hipStream_t stream) {
     const dim3 grid(groups), block(64 * flash_small::kWaves);
     const bool bf16 = p.cache_dtype == HIPATTN_BF16;
-    if (p.cache_dtype == HIPATTN_U8) {
+    if (p.cache_dtype == HIPATTN_I8) {
+        if (p.head_dim <= 64)
+            hipLaunchKernelGGL((flash_small::paged_tiles_kernel<false, 64, true, 64, true>), grid, block, 0, stream, p);
+        else if (p.head_dim <= 96)
+            hipLaunchKernelGGL((flash_small::paged_tiles_kernel<false, 128, true, 96, true>), grid, block, 0, stream, p);
+        else if (p.head_dim <= 128)
+            hipLaunchKernelGGL((flash_small::paged_tiles_kernel<false, 128, true, 128, true>), grid, block, 0, stream, p);
+        else
+            hipLaunchKernelGGL((flash_small::paged_tiles_kernel<false, 256, true, 256, true>), grid, block, 0, stream, p);
+    } else if (p.cache_dtype == HIPATTN_U8) {
         if (p.head_dim <= 64)
             hipLaunchKernelGGL((flash_small::paged_tiles_kernel<false, 64, true>), grid, block, 0, stream, p);
         else if (p.head_dim <= 96)
@@ -777,7 +812,7 @@ bool paged_tiles_supported(const PagedParams& p) {
     return p.head_dim >= 8 && p.head_dim <= 256 && p.head_dim % 8 == 0 && G <= flash_small::kTileQ &&
            p.block_size > 0 && (p.block_size & (p.block_size - 1)) == 0 &&
            (p.q_dtype == HIPATTN_F16 || p.q_dtype == HIPATTN_BF16) &&
-           (p.cache_dtype == HIPATTN_F16 || p.cache_dtype == HIPATTN_BF16 || p.cache_dtype == HIPATTN_U8) && aligned16(p.q) && aligned16(p.key_cache) &&
+           (p.cache_dtype == HIPATTN_F16 || p.cache_dtype == HIPATTN_BF16 || eight_bit(p.cache_dtype)) && aligned16(p.q) && aligned16(p.key_cache) &&
            aligned16(p.value_cache) && ((uintptr_t)p.out % (p.out_dtype == HIPATTN_F32 ? 16 : 8)) == 0;
 }
 

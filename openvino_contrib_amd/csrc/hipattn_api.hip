@@ -669,6 +669,7 @@ hipattn_status paged_attention_impl(const hipattn_pa_desc* desc, const void* q, 
         HIP_TRY(hipattn::launch_paged_fast(p, do_write ? &w : nullptr, as_stream(stream), g_probe));
     } else if (!forced_generic && hipattn::paged_tiles_supported(p)) {
         if (hipattn_status st = take_workspace(hipattn::paged_tiles_workspace_bytes(p))) return st;
+        HIP_TRY(write_i8());
         g_kernel_path = "paged_mfma_tiles";
         if (do_write) HIP_TRY(hipattn::launch_kv_cache_write(w, as_stream(stream)));
         HIP_TRY(hipattn::launch_paged_tiles(p, workspace, as_stream(stream), g_probe));

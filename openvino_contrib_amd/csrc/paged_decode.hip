@@ -77,7 +77,7 @@ __device__ __forceinline__ void plan_block(const PagedParams& p) {
         // one of the flash kernel does a 128-row x 64-key tile of one head in about 1.1 us
         // (u8 caches, dequantised on the way: 1.4 us).  Each part gets compute units in
         // proportion to its work, so that both end together.
-        const bool u8 = p.cache_dtype == HIPATTN_U8;
+        const bool u8 = eight_bit(p.cache_dtype);
         const float decode_us = (float)total_blk * p.num_heads_kv * (u8 ? 8704.0f / 24000.0f : 16384.0f / 33000.0f) * p.overlap_share;
         const float prefill_us = total_keys * p.num_heads_q * (u8 ? 1.4f : 1.1f);
         const int cus = p.num_waves >> 3;
@@ -204,9 +204,9 @@ __device__ __forceinline__ void merge_segment_head(const PagedParams& p, const L
     }
 }
 
-template <bool kU8, bool kBf16, int kWaves, bool kSelfPlan = false, int kHD = kD, int kBlk = kBS, bool kPad = false, bool kAlibi = false, bool kHalfFromBf16 = false>
+template <bool kU8, bool kBf16, int kWaves, bool kSelfPlan = false, int kHD = kD, int kBlk = kBS, bool kPad = false, bool kAlibi = false, bool kHalfFromBf16 = false, bool kI8 = false>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_decode_kernel(PagedParams p, KvWriteParams wp, int do_write) {
-    paged_decode_body<kU8, kBf16, kWaves, kSelfPlan, kHD, kBlk, kPad, kAlibi, kHalfFromBf16>(p, wp, do_write, (int)blockIdx.x);
+    paged_decode_body<kU8, kBf16, kWaves, kSelfPlan, kHD, kBlk, kPad, kAlibi, kHalfFromBf16, kI8>(p, wp, do_write, (int)blockIdx.x);
 }
 
 // ---- head size 256 ------------------------------------------------------------------------------
@@ -825,7 +825,9 @@ bool paged_fast_supported(const PagedParams& p) {
     if (p.alibi_slopes && p.head_dim > 128) return false;  // (the head-256 decode kernel has no distance term: the query-tile kernel takes the batch)
     // (above 128: paged_decode256_kernel)
     return p.head_dim >= 8 && p.head_dim <= 256 && p.head_dim % 8 == 0 &&
-           (p.cache_dtype == HIPATTN_F16 || p.cache_dtype == HIPATTN_BF16 || p.cache_dtype == HIPATTN_U8);
+           (p.cache_dtype == HIPATTN_F16 || p.cache_dtype == HIPATTN_BF16 || p.cache_dtype == HIPATTN_U8 ||
+            // (i8: neither the head-256 decode kernel nor one with the distance bias is built)
+            (p.cache_dtype == HIPATTN_I8 && p.head_dim <= 128 && !p.alibi_slopes));
 }
 
 PagedParams split_kv_heads(const PagedParams& p) {
@@ -889,7 +891,7 @@ static int plan_rows(const PagedParams& p) { return query_tile_bound(p) == 0 ? p
 static bool overlap_wanted(const PagedParams& p) {
     if (query_tile_bound(p) == 0 || p.num_waves > 0 || p.no_side_stream || p.alibi_slopes || half_operands_from_bf16(p)) return false;
     // the eight-wavefront decode kernel: head size 128, and 16-bit caches at the head sizes between 64 and 128
-    if (p.head_dim != kD && !(p.head_dim > 64 && p.head_dim < kD && p.cache_dtype != HIPATTN_U8)) return false;
+    if (p.head_dim != kD && !(p.head_dim > 64 && p.head_dim < kD && !eight_bit(p.cache_dtype))) return false;
     return option(kOptMixedOverlap) != 0;
 }
 
@@ -900,7 +902,7 @@ static int choose_num_waves(const PagedParams& p, bool overlap) {
     // (u8 at head size 64 has the most arithmetic per byte of all: every resident wavefront, 0.59 against
     // 0.48 of HBM peak with six per compute unit on the 128-sequence u8 batch)
     if (p.head_dim > 128) return resident;  // half as many bytes in flight per wavefront: twice the wavefronts
-    if (p.cache_dtype == HIPATTN_U8) return p.head_dim <= 64 ? resident : resident / 4 * 3;
+    if (eight_bit(p.cache_dtype)) return p.head_dim <= 64 ? resident : resident / 4 * 3;
     return resident / 2;
 }
 
@@ -981,7 +983,7 @@ void paged_fast_plan(PagedParams& p, void* workspace, size_t workspace_bytes) {
     const int64_t segments = (int64_t)p.num_rows * p.num_heads_kv;
     // 16-bit caches: from 128 segments on all wavefronts (24 sequences of 400: 16.1 us against 17.4 with 512; 63 of 300, 504
     // segments: 23.1 against 23.8 with 768).  (On-demand pieces: every ticket group needs its wavefronts.)
-    const bool all = fixed_waves || option(kOptDynPieces) > 0 || overlap || (p.cache_dtype != HIPATTN_U8 && segments >= 128);
+    const bool all = fixed_waves || option(kOptDynPieces) > 0 || overlap || (!eight_bit(p.cache_dtype) && segments >= 128);
     p.few_waves = all ? 0 : (int)std::max<int64_t>(512, 2 * segments);
     const size_t slots = (size_t)p.num_waves + p.dyn_pieces + (size_t)p.num_rows * p.num_heads_kv;
     uint8_t* w = (uint8_t*)workspace;
@@ -1019,7 +1021,7 @@ void paged_fast_plan(PagedParams& p, void* workspace, size_t workspace_bytes) {
     // 60 tokens 35.5 against 44.5).
     const bool few_pieces = fixed_waves || most_blocks(p) <= (overlap ? 8 : segments >= 128 ? 4 : 2) ||
                             2 * most_waves(p) <= (p.head_dim <= 64 ? 5 : 6) * segments;
-    p.fused_merge = (option(kOptFusedMerge) != 0 && p.cache_dtype == HIPATTN_U8 && p.dyn_pieces == 0 && p.head_dim <= 128 && few_pieces) ? 1 : 0;
+    p.fused_merge = (option(kOptFusedMerge) != 0 && eight_bit(p.cache_dtype) && p.dyn_pieces == 0 && p.head_dim <= 128 && few_pieces) ? 1 : 0;
     p.merge_tag = next_merge_tag();
 }
 
@@ -1165,6 +1167,18 @@ static void launch_decode_blk(const PagedParams& p, const KvWriteParams& wp, int
     }
 }
 
+// The i8 forms.
+template <int kWaves, bool kSelfPlan, int kHD, bool kPad>
+static void launch_decode_i8(const PagedParams& p, dim3 grid, dim3 block, hipStream_t stream) {
+    const KvWriteParams none{};
+    if (p.block_size == 32)
+        hipLaunchKernelGGL((paged_decode_kernel<true, false, kWaves, kSelfPlan, kHD, 32, kPad, false, false, true>), grid, block, 0, stream, p, none, 0);
+    else if (p.block_size == 16)
+        hipLaunchKernelGGL((paged_decode_kernel<true, false, kWaves, kSelfPlan, kHD, 16, kPad, false, false, true>), grid, block, 0, stream, p, none, 0);
+    else if constexpr (!kSelfPlan)
+        hipLaunchKernelGGL((paged_decode_kernel<true, false, kWaves, false, kHD, 0, kPad, false, false, true>), grid, block, 0, stream, p, none, 0);
+}
+
 template <bool kBf16, bool kPad, bool kU8 = false>
 static void launch_decode256_blk(const PagedParams& p, dim3 grid, dim3 block, hipStream_t stream) {
     if (p.block_size == 32)
@@ -1179,6 +1193,19 @@ template <int kWaves, bool kSelfPlan>
 static void launch_decode(const PagedParams& p, const KvWriteParams& wp, int do_write, dim3 grid, dim3 block,
                           hipStream_t stream) {
     const bool bf16 = p.cache_dtype == HIPATTN_BF16, u8 = p.cache_dtype == HIPATTN_U8;
+    if (p.cache_dtype == HIPATTN_I8) {
+        if (p.head_dim == 128)
+            launch_decode_i8<kWaves, kSelfPlan, 128, false>(p, grid, block, stream);
+        else if constexpr (kWaves == 1 && !kSelfPlan) {
+            if (p.head_dim == 64)
+                launch_decode_i8<1, false, 64, false>(p, grid, block, stream);
+            else if (p.head_dim > 64)
+                launch_decode_i8<1, false, 128, true>(p, grid, block, stream);
+            else
+                launch_decode_i8<1, false, 64, true>(p, grid, block, stream);
+        }
+        return;
+    }
     if (p.head_dim == 128) {
         if (u8)
             launch_decode_blk<true, false, kWaves, kSelfPlan, 128, false>(p, wp, do_write, grid, block, stream);

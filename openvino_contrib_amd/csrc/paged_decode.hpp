@@ -310,6 +310,52 @@ __device__ __forceinline__ void load_block_padded(BlockRegs<kU8>& b, const uint8
     }
 }
 
+// A unit of an i8 cache: rows of head_dim codes and nothing between them.  The blocks' scales travel as wavefront-uniform
+// values beside it (UnitScales).
+struct BlockRegsI8 {
+    uint2_t k[2][4];  // as BlockRegs<true>
+    uint2_t v[8];
+};
+// What a tile's block contributes to its scores and probabilities: the key scale times softmax scale and log2(e), log2 of the
+// value scale, and its reciprocal.
+struct UnitScales {
+    float key[2], value_log2[2], value_inverse[2];
+};
+
+// row: bytes from row to row (kHD unless the head is narrower); koff, voff, v_ok as in load_block_padded.
+template <int kHD, int kBlk, bool kPad>
+__device__ __forceinline__ void load_block_i8(BlockRegsI8& b, const uint8_t* const (&kb)[2], const uint8_t* const (&vb)[2], int row,
+                                              const int (&koff)[kHD / 32], int voff, bool v_ok, int n16, int kg) {
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        if constexpr (kPad) {
+            const uint8_t* const kt = kBlk == 32 ? kb[0] + t * 16 * row : kb[t];
+#pragma unroll
+            for (int i = 0; i < kHD / 32; i++) b.k[t][i] = *(const uint2_t*)(kt + koff[i]);
+        } else {  // a lane's kHD / 4 codes of a row lie side by side
+            const uint8_t* const kt = (kBlk == 32 ? kb[0] + t * 16 * kHD : kb[t]) + n16 * kHD + kg * (kHD / 4);
+#pragma unroll
+            for (int i = 0; i < kHD / 32; i += 2) {
+                const uint4_t w = *(const uint4_t*)(kt + i * 8);
+                b.k[t][i] = (uint2_t){w[0], w[1]};
+                b.k[t][i + 1] = (uint2_t){w[2], w[3]};
+            }
+        }
+    }
+    const bool mine = kPad ? v_ok : (kHD == 128 || n16 * 8 < kHD);
+    const int first = kPad ? voff : kg * 4 * kHD + n16 * 8, step = kPad ? row : kHD;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        const uint8_t* const vt = (kBlk == 32 ? vb[0] + t * 16 * step : vb[t]) + first;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            uint2_t piece = {0u, 0u};
+            if (mine) piece = *(const uint2_t*)(vt + r * step);
+            b.v[t * 4 + r] = piece;
+        }
+    }
+}
+
 struct WaveState {
     float m;          // running max of the scaled scores (log2 domain), per head (lane & 15)
     float l;          // this lane's share of the running sum
@@ -471,6 +517,86 @@ __device__ __forceinline__ void process_block(WaveState& st, BlockRegs<kU8>& b, 
     }
 }
 
+
+// A unit of an i8 cache.  Codes become the exact fp16 integers 1024 + 128 + code (the sign bit flipped, then as the u8 bytes), so
+// that scores are off by 1152 sum(q) and outputs by 1152 sum(p): one constant per head, taken out of the scores here and of
+// the outputs when the segment is done.  A tile is one block's, so its two scales are one number each:
+//   score * log2(e) = (s - 1152 sum(q)) key,  key = key scale * softmax scale * log2(e)
+//   v_scale exp2(score - reference) = exp2(score + log2(v_scale) - reference)
+// The value scale joins the exponent: the running maximum then bounds what is multiplied with the codes, in fp16 whatever the
+// scales' size, and the row sum takes the probabilities back by 1 / v_scale.  (A u8 row's scale and zero-point cost the u8 form
+// two broadcasts and two more operations for every probability.)
+constexpr float kCodeBias = kByteBias + 128.0f;
+template <int kHD, bool kTileMask>
+__device__ __forceinline__ void process_block_i8(WaveState& st, BlockRegsI8& b, const half8_t (&qf)[4], float sumq, const UnitScales& u, int tok_base,
+                                                 int j0, int ctx, int kg, int tiles_in) {
+    const int tiles = kTileMask ? tiles_in : 3;
+    using Op = Op16<false>;
+    float4_t s[2];
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        s[t] = (float4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kHD / 32; i++) {
+            const uint32_t lo = b.k[t][i][0] ^ 0x80808080u, up = b.k[t][i][1] ^ 0x80808080u;
+            uint4_t w;
+            w[0] = bytes_to_biased_half2(lo, 0x04010400u);
+            w[1] = bytes_to_biased_half2(lo, 0x04030402u);
+            w[2] = bytes_to_biased_half2(up, 0x04010400u);
+            w[3] = bytes_to_biased_half2(up, 0x04030402u);
+            s[t] = Op::mma(Op::from_bits(w), qf[i], s[t]);
+        }
+    }
+    const bool partial = (tok_base < j0) || (tok_base + kUnit > ctx) || tiles != 3;  // wavefront-uniform
+    float sv[8];
+    float mloc = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        const float off = fmaf(-kCodeBias * sumq, u.key[t], u.value_log2[t]);
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            float x = fmaf(s[t][r], u.key[t], off);
+            if (partial) {
+                const int tok = tok_base + t * 16 + kg * 4 + r;
+                x = (tok >= j0 && tok < ctx && ((tiles >> t) & 1)) ? x : -INFINITY;
+            }
+            sv[t * 4 + r] = x;
+            mloc = fmaxf(mloc, x);
+        }
+    }
+    mloc = max_over_rows(mloc);
+    const float m_new = fmaxf(st.m, mloc);  // finite: every processed block holds an attended token
+    const float alpha = fast_exp2(st.m - m_new);
+    st.m = m_new;
+    half8_t pf;
+    float csum = 0.0f, lsum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float pj = fast_exp2(sv[j] - m_new);
+        lsum[j >> 2] += pj;
+        Op::set(pf, j, pj);
+        csum += Op::get(pf, j);
+    }
+    st.l = st.l * alpha + fmaf(lsum[0], u.value_inverse[0], lsum[1] * u.value_inverse[1]);
+    st.corr = st.corr * alpha + csum;
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) st.acc[e] *= alpha;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        b.v[j][0] ^= 0x80808080u;
+        b.v[j][1] ^= 0x80808080u;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        uint4_t w;
+        const uint32_t sel = 0x0c000c00u | ((4u + (e & 3)) << 16) | (uint32_t)(e & 3);
+#pragma unroll
+        for (int jp = 0; jp < 4; jp++) w[jp] = bytes_to_biased_half2(b.v[2 * jp][e >> 2], b.v[2 * jp + 1][e >> 2], sel);
+        st.acc[e] = Op::mma(Op::from_bits(w), pf, st.acc[e]);
+    }
+}
 
 // Length of one (sequence, kv head) segment on the work line: its blocks plus `switch_cost`
 // units that stand for the time a wavefront loses when it starts on a new segment (dependent
@@ -688,11 +814,13 @@ constexpr int kSelfPlanMaxRows = 256;
 // head sizes between 64 and 128, kPad), the self-planning form on blocks of 32 or 16 only.
 // kPad: the call's head size (p.head_dim, a multiple of 8) may be smaller than kHD: the missing columns of
 // Q are zeros and those of V are not read.
-template <bool kU8, bool kBf16, int kWaves, bool kSelfPlan = false, int kHD = kD, int kBlk = kBS, bool kPad = false, bool kAlibi = false, bool kHalfFromBf16 = false>
+template <bool kU8, bool kBf16, int kWaves, bool kSelfPlan = false, int kHD = kD, int kBlk = kBS, bool kPad = false, bool kAlibi = false, bool kHalfFromBf16 = false, bool kI8 = false>
 __device__ __forceinline__ void paged_decode_body(const PagedParams& p, const KvWriteParams& wp, int do_write, int workgroup) {
     // kHalfFromBf16: the cache holds bf16, the operands are fp16 (fp16 queries): blocks are converted as they arrive
     static_assert(!kHalfFromBf16 || (!kU8 && !kBf16 && kWaves == 1 && !kSelfPlan && kHD == 128 && !kPad && !kAlibi), "bf16 blocks as fp16 operands: the ordinary launch at head size 128 only");
     static_assert(!kAlibi || (kWaves == 1 && !kSelfPlan), "the distance bias (p.alibi_slopes) exists in the ordinary launch only");
+    // kI8: a cache of codes with a scale per block and kv head; it shares what holds for both 8-bit caches (kU8)
+    static_assert(!kI8 || (kU8 && !kAlibi), "i8 caches: an 8-bit form, without the distance bias");
     // The merge inside the kernel (p.fused_merge) is built into the u8 instantiations only: the 16-bit ones use
     // every register in their loop, and with that code behind the loop the allocator spilled 29 of them.
     constexpr bool kFusedBuilt = kU8;
@@ -760,9 +888,10 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams& p, const Kv
     if (w >= num_waves) return;
     const Line line(total, num_waves, p.dyn_pieces);
 
-    constexpr int64_t kRowBytesBuilt = kU8 ? (kHD + 8) : (2 * kHD);
+    constexpr int kRowHead = kU8 && !kI8 ? 8 : 0;  // bytes ahead of a row's payload
+    constexpr int64_t kRowBytesBuilt = kU8 ? (kHD + kRowHead) : (2 * kHD);
     const int head_dim = kPad ? p.head_dim : kHD;                       // (a constant unless kPad)
-    const int64_t kRowBytes = kPad ? (kU8 ? p.head_dim + 8 : 2 * p.head_dim) : kRowBytesBuilt;
+    const int64_t kRowBytes = kPad ? (kU8 ? p.head_dim + kRowHead : 2 * p.head_dim) : kRowBytesBuilt;
     const int64_t block_stride = (int64_t)(Hkv / p.kv_share) * blk * kRowBytes;  // (kv_share: see PagedParams)
     // kPad: this lane's K piece offsets, V offset and whether its V columns exist
     int koff[kHD / 32];
@@ -772,9 +901,9 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams& p, const Kv
 #pragma unroll
         for (int i = 0; i < kHD / 32; i++) {
             const int first = kg * (kHD / 4) + i * 8;  // first of the piece's eight columns
-            koff[i] = n16 * (int)kRowBytes + (kU8 ? 8 + (first < head_dim ? first : 0) : (first < head_dim ? first * 2 : 0));
+            koff[i] = n16 * (int)kRowBytes + (kU8 ? kRowHead + (first < head_dim ? first : 0) : (first < head_dim ? first * 2 : 0));
         }
-        voff = kg * 4 * (int)kRowBytes + (kU8 ? 8 + n16 * 8 : n16 * 16);
+        voff = kg * 4 * (int)kRowBytes + (kU8 ? kRowHead + n16 * 8 : n16 * 16);
         v_ok = n16 * 8 < head_dim;
     }
 
@@ -843,7 +972,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams& p, const Kv
         const int64_t head_off = (int64_t)h_kv * blk * kRowBytes;
         const int sub_shift = kBlk ? 0 : __builtin_ctz(p.block_size >> 5);
 
-        if constexpr (kSelfPlan) {
+        if constexpr (kSelfPlan && !kI8) {
             // The new tokens of this call whose cache rows this piece is about to read go into the cache
             // first: the row's own token (in the segment's last block) and, when its sequence
             // contributes several tokens to the batch, the tokens ahead of it.  The same wavefront
@@ -897,8 +1026,34 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams& p, const Kv
             const int gn = min(kGroup, n - g0);
             const int my_entry = kBlk ? g0 * kEntries + lane : (lb0 + g0 + lane) >> sub_shift;
             const int my_pb = (lane < gn * kEntries && my_entry < entries) ? table[my_entry] : -1;
+            // kI8: what the scales of this lane's entry make of its tiles; blocks of zeros get a scale too small to count
+            float my_key = 0.0f, my_value_log2 = 0.0f, my_value_inverse = 1.0f;
+            if constexpr (kI8) {
+                if (my_pb >= 0 && my_pb < p.num_blocks) {
+                    const int64_t at = (int64_t)my_pb * (Hkv / p.kv_share) + h_kv;
+                    const float value = fmaxf(p.value_scales[at], 0x1p-100f);
+                    my_key = p.key_scales[at] * c;
+                    my_value_log2 = __builtin_amdgcn_logf(value);
+                    my_value_inverse = 1.0f / value;
+                }
+            }
+            const auto lane_of = [](float x, int i) __attribute__((always_inline)) {
+                return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i));
+            };
+            const auto scales_of = [&](int i) __attribute__((always_inline)) {
+                UnitScales u;
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    const int entry = kEntries == 2 ? 2 * i + t : i;
+                    u.key[t] = lane_of(my_key, entry);
+                    u.value_log2[t] = lane_of(my_value_log2, entry);
+                    u.value_inverse[t] = lane_of(my_value_inverse, entry);
+                }
+                return u;
+            };
+            using Regs = typename std::conditional<kI8, BlockRegsI8, BlockRegs<kU8>>::type;
             // which tiles of unit i were issued (0: none, the unit is skipped); never reads outside the cache
-            auto issue = [&](BlockRegs<kU8>& regs, int i) -> int {
+            auto issue = [&](Regs& regs, int i) -> int {
                 if constexpr (kEntries == 1) {
                     const int pb = __builtin_amdgcn_readlane(my_pb, i);
                     if (pb < 0 || pb >= p.num_blocks) return 0;
@@ -906,7 +1061,9 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams& p, const Kv
                     if constexpr (kBlk == 0) off += (int64_t)((lb0 + g0 + i) & sub_mask) * (kUnit * kRowBytes);
                     const uint8_t* const kb[2] = {p.key_cache + off, p.key_cache + off + 16 * kRowBytes};
                     const uint8_t* const vb[2] = {p.value_cache + off, p.value_cache + off + 16 * kRowBytes};
-                    if constexpr (kPad)
+                    if constexpr (kI8)
+                        load_block_i8<kHD, kTileBlk, kPad>(regs, kb, vb, (int)kRowBytes, koff, voff, v_ok, n16, kg);
+                    else if constexpr (kPad)
                         load_block_padded<kU8, kHD, kTileBlk>(regs, kb, vb, (int)kRowBytes, koff, voff, v_ok, n16, kg);
                     else
                         load_block<kU8, kHD, kTileBlk>(regs, kb, vb, n16, kg);
@@ -925,7 +1082,9 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams& p, const Kv
                     const int64_t off1 = (int64_t)((ok & 2) ? pb1 : pb0) * block_stride + head_off;
                     const uint8_t* const kb[2] = {p.key_cache + off0, p.key_cache + off1};
                     const uint8_t* const vb[2] = {p.value_cache + off0, p.value_cache + off1};
-                    if constexpr (kPad)
+                    if constexpr (kI8)
+                        load_block_i8<kHD, kTileBlk, kPad>(regs, kb, vb, (int)kRowBytes, koff, voff, v_ok, n16, kg);
+                    else if constexpr (kPad)
                         load_block_padded<kU8, kHD, kTileBlk>(regs, kb, vb, (int)kRowBytes, koff, voff, v_ok, n16, kg);
                     else
                         load_block<kU8, kHD, kTileBlk>(regs, kb, vb, n16, kg);
@@ -952,7 +1111,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams& p, const Kv
                 // consumed.  (Measured on the 128-sequence u8 workload: two stages 452 us, three 455 us,
                 // four spill registers and fall to 629 us.)
                 constexpr int kStages = HIPATTN_U8_STAGES;
-                BlockRegs<kU8> regs[kStages];
+                Regs regs[kStages];
                 int ok[kStages];
 #pragma unroll
                 for (int u = 0; u < kStages - 1; u++) ok[u] = (u < gn) ? issue(regs[u], u) : 0;
@@ -964,7 +1123,11 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams& p, const Kv
                         constexpr int kLast = kStages - 1;
                         ok[(u + kLast) % kStages] =
                             (idx + kLast < gn) ? issue(regs[(u + kLast) % kStages], idx + kLast) : 0;
-                        if (ok[u]) process_block<kU8, kBf16, kHD, kEntries != 1, kAlibi>(st, regs[u], qf, sumq, c, (lb0 + g0 + idx) * kUnit, rg.j0, rg.ctx, kg, ok[u], slopes, G);
+                        if constexpr (kI8) {
+                            if (ok[u]) process_block_i8<kHD, kEntries != 1>(st, regs[u], qf, sumq, scales_of(idx), (lb0 + g0 + idx) * kUnit, rg.j0, rg.ctx, kg, ok[u]);
+                        } else {
+                            if (ok[u]) process_block<kU8, kBf16, kHD, kEntries != 1, kAlibi>(st, regs[u], qf, sumq, c, (lb0 + g0 + idx) * kUnit, rg.j0, rg.ctx, kg, ok[u], slopes, G);
+                        }
                     }
                 }
             }
@@ -977,6 +1140,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams& p, const Kv
         if constexpr (kU8) {
             corr += __shfl_xor(corr, 16, 64);
             corr += __shfl_xor(corr, 32, 64);
+            if constexpr (kI8) corr *= kCodeBias;
         }
         const int64_t slot = (int64_t)piece + (int64_t)s * Hkv + h;  // unique per (piece, segment)
         if (n16 < G) {

@@ -14,29 +14,29 @@ namespace hipattn {
 
 namespace {
 
-template <bool kU8, bool kBf16, int kBlk, bool kPad>
+template <bool kU8, bool kBf16, int kBlk, bool kPad, bool kI8 = false>
 __global__ __launch_bounds__(flash::kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_mixed_kernel(PagedParams p, int decode_workgroups,
                                                                                                                 int chunk_heads_kv) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[flash::kLdsBytes];
     if ((int)blockIdx.x < decode_workgroups) {
         const KvWriteParams none{};
-        paged_decode_body<kU8, kBf16, 8, false, kD, kBlk, kPad>(p, none, 0, (int)blockIdx.x);
+        paged_decode_body<kU8, kBf16, 8, false, kD, kBlk, kPad, false, false, kI8>(p, none, 0, (int)blockIdx.x);
         return;
     }
     p.num_heads_kv = chunk_heads_kv;
     p.kv_share = 1;
-    flash::paged_prefill_item<kBf16, kU8, kPad, kU8>(p, (int)blockIdx.x - decode_workgroups, lds);
+    flash::paged_prefill_item<kBf16, kU8, kPad, kU8 && !kI8, kI8>(p, (int)blockIdx.x - decode_workgroups, lds);
 }
 
-template <bool kU8, bool kBf16, bool kPad>
+template <bool kU8, bool kBf16, bool kPad, bool kI8 = false>
 void launch_blk(const PagedParams& p, int decode_workgroups, int chunk_heads_kv, dim3 grid, hipStream_t stream) {
     const dim3 block(flash::kThreads);
     if (p.block_size == 32)
-        hipLaunchKernelGGL((paged_mixed_kernel<kU8, kBf16, 32, kPad>), grid, block, 0, stream, p, decode_workgroups, chunk_heads_kv);
+        hipLaunchKernelGGL((paged_mixed_kernel<kU8, kBf16, 32, kPad, kI8>), grid, block, 0, stream, p, decode_workgroups, chunk_heads_kv);
     else if (p.block_size == 16)
-        hipLaunchKernelGGL((paged_mixed_kernel<kU8, kBf16, 16, kPad>), grid, block, 0, stream, p, decode_workgroups, chunk_heads_kv);
+        hipLaunchKernelGGL((paged_mixed_kernel<kU8, kBf16, 16, kPad, kI8>), grid, block, 0, stream, p, decode_workgroups, chunk_heads_kv);
     else
-        hipLaunchKernelGGL((paged_mixed_kernel<kU8, kBf16, 0, kPad>), grid, block, 0, stream, p, decode_workgroups, chunk_heads_kv);
+        hipLaunchKernelGGL((paged_mixed_kernel<kU8, kBf16, 0, kPad, kI8>), grid, block, 0, stream, p, decode_workgroups, chunk_heads_kv);
 }
 
 }  // namespace
@@ -46,7 +46,7 @@ void launch_blk(const PagedParams& p, int decode_workgroups, int chunk_heads_kv,
 bool paged_mixed_supported(const PagedParams& p) {
     if (p.sinks || p.alibi_slopes) return false;
     if (p.head_dim == kD) return true;
-    return p.cache_dtype != HIPATTN_U8 && (((uintptr_t)p.q | (uintptr_t)p.key_cache | (uintptr_t)p.value_cache | (uintptr_t)p.out) & 15) == 0;
+    return !eight_bit(p.cache_dtype) && (((uintptr_t)p.q | (uintptr_t)p.key_cache | (uintptr_t)p.value_cache | (uintptr_t)p.out) & 15) == 0;
 }
 
 hipError_t launch_paged_mixed(const PagedParams& p, int chunk_heads_kv, hipStream_t stream) {
@@ -55,7 +55,9 @@ hipError_t launch_paged_mixed(const PagedParams& p, int chunk_heads_kv, hipStrea
     const int G = p.num_heads_q / chunk_heads_kv;
     const dim3 grid((unsigned)(decode_workgroups + (int64_t)p.max_q_tiles * ((G & 1) == 0 ? p.num_heads_q / 2 : p.num_heads_q)));
     const bool bf16 = p.cache_dtype == HIPATTN_BF16;
-    if (p.cache_dtype == HIPATTN_U8)
+    if (p.cache_dtype == HIPATTN_I8)
+        launch_blk<true, false, false, true>(p, decode_workgroups, chunk_heads_kv, grid, stream);
+    else if (p.cache_dtype == HIPATTN_U8)
         launch_blk<true, false, false>(p, decode_workgroups, chunk_heads_kv, grid, stream);
     else if (p.head_dim == kD)
         bf16 ? launch_blk<false, true, false>(p, decode_workgroups, chunk_heads_kv, grid, stream)
