@@ -327,7 +327,7 @@ hipattn_status hipattn_rotate_key_cache(const hipattn_pa_desc* desc, void* key_c
  * them), and so is the workspace (hipattn_paged_attention_workspace_size).  No counterpart in the reference.
  * The calls that write such a cache (this one without HIPATTN_PA_SKIP_CACHE_WRITE, and hipattn_rope_append) keep the scales up to
  * date.  With a = the largest magnitude among the rows that one call writes into the block for the head,
- *     scale' = max(scale before, a / 127)      (scale before: 0 when the call writes the block's row 0; a / 127 below 1e-30: 0)
+ *     scale' = max(scale before, a * (1 / 127))   (scale before: 0 when the call writes the block's row 0; a product below 1e-30: 0)
  *     code   = clamp(rint(x * (1 / scale')), -127, 127)                              for the new rows
  *     code'  = rint(code * (scale before / scale'))       for the rows that precede them, when the scale has grown
  * in fp32, every operation rounded by itself; codes are 0 where the scale is.  Rows behind the new ones keep their bytes.

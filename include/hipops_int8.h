@@ -16,8 +16,8 @@ extern "C" {
 #endif
 
 /* ---- rows as 8-bit codes with a scale each ----------------------------------------------------
- * codes[r, i] = clamp(rint(y[r, i] * (1 / scales[r])), -127, 127), scales[r] = max_i |y[r, i]| / 127, all in fp32; a scale below
- * 1e-30 is 0, and so are its codes.  y is one of
+ * codes[r, i] = clamp(rint(y[r, i] * (1 / scales[r])), -127, 127), scales[r] = max_i |y[r, i]| * (1 / 127), all in fp32; a scale
+ * below 1e-30 is 0, and so are its codes.  y is one of
  *   HIPOPS_QUANTIZE_PLAIN      x[r, i]
  *   HIPOPS_QUANTIZE_RMS_NORM   x[r, i] * 1/sqrt(mean_i(x[r, i]^2) + eps) * gamma[i]   (gamma [width], or NULL: ones)
  *   HIPOPS_QUANTIZE_GLU        act(x[r, g + i]) * x[r, u + i], rows of x 2 * width long, as hipops_glu

@@ -24,7 +24,7 @@ struct QuantizeParams {
 constexpr int kMaxWaves = 16;
 
 __device__ __forceinline__ float scale_of_peak(float peak) {
-    const float s = peak / 127.0f;
+    const float s = peak * (1.0f / 127.0f);
     return s < 1e-30f ? 0.0f : s;
 }
 __device__ __forceinline__ int code_of(float y, float inverse) { return (int)fminf(fmaxf(rintf(y * inverse), -127.0f), 127.0f); }

@@ -27,7 +27,7 @@ def rotated(x, cos, sin, rotary, interleaved):
 
 
 def scale_of_peak(peak):
-    s = (np.asarray(peak, np.float32) / np.float32(127)).astype(np.float32)
+    s = (np.asarray(peak, np.float32) * (one / np.float32(127))).astype(np.float32)
     return np.where(s < np.float32(1e-30), np.float32(0), s)
 
 
