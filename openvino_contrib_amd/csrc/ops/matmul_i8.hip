@@ -1,55 +1,77 @@
-// Products of 8-bit codes (hipops_matmul_i8): c = a_scale b_scale (A B^T) + bias + residual on v_mfma_i32_32x32x32_i8, sums exact in
-// 32-bit integers.
+// Products of 8-bit codes (hipops_matmul_i8): c = a_scale b_scale (A B^T) + bias + residual, sums exact in 32-bit integers on the
+// matrix cores.  The entry, the choice among the kernels, and the one for up to 16 activation rows; the others: matmul_i8_tiles.hip.
+#include <algorithm>
+#include <cmath>
+
 #include "ops/matmul_i8.hpp"
 
 namespace hipops {
 
 namespace {
 
-// The plain kernel: any strides, alignment and k.  Four wavefronts, a tile of 64 x 64, 64 bytes of k at a time through LDS.
-constexpr int kPlainTile = 64, kPlainK = 64;
+// Up to 16 activation rows: the weights, read once, are all of the time.  A workgroup takes 16 weight rows and its eight wavefronts an
+// eighth of k each; a lane's loads are the matrix operands as they stand (16 bytes of k of weight row lane % 16, activations
+// alike), kGroup steps multiplied while the next ones are on their way.  Only the eight partial sums meet in LDS.
+constexpr int kFewWaves = 8, kFewGroup = 4;
 
-__device__ __forceinline__ uint4_t load_codes16(const int8_t* row, int64_t at, int64_t k, bool there, bool aligned) {
-    if (!there || at >= k) return (uint4_t){0u, 0u, 0u, 0u};
-    if (aligned && at + 16 <= k) return *(const uint4_t*)(row + at);
-    uint4_t w = {0u, 0u, 0u, 0u};
+__global__ __launch_bounds__(64 * kFewWaves) void matmul_i8_few_kernel(MatmulI8Params p) {
+    __shared__ int4_t sums[kFewWaves][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, row = lane & 15, quarter = lane >> 4;
+    const int64_t n0 = 16 * (int64_t)blockIdx.x;
+    const int steps = (int)((p.k + 63) / 64);
+    const int first = steps * wave / kFewWaves, last = steps * (wave + 1) / kFewWaves;
+    const int8_t* const w = p.b + min(n0 + row, p.n - 1) * p.ldb + 16 * quarter;
+    const int8_t* const x = p.a + (int64_t)min((int64_t)row, p.m - 1) * p.lda + 16 * quarter;
+    const bool real = row < p.m;
+    const int whole = (int)((p.k - 16 * quarter + 48) / 64);  // steps in which this lane has a piece (k is a multiple of 16)
+    int4_t acc = {0, 0, 0, 0};
+    struct Group {
+        uint4_t w[kFewGroup], x[kFewGroup];
+    } now, next;
+    const auto load = [&](Group& g, int s) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < 16; e++)
-        if (at + e < k) w[e >> 2] |= (uint32_t)(uint8_t)row[at + e] << (8 * (e & 3));
-    return w;
-}
-
-__global__ __launch_bounds__(256) void matmul_i8_plain_kernel(MatmulI8Params p, int aligned) {
-    __shared__ uint4_t tile[2][kPlainTile][kPlainK / 16];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t m0 = (int64_t)blockIdx.y * kPlainTile, n0 = (int64_t)blockIdx.x * kPlainTile;
-    const int row = threadIdx.x >> 2, piece = threadIdx.x & 3;
-    const int8_t* const a = p.a + (m0 + row) * p.lda;
-    const int8_t* const b = p.b + (n0 + row) * p.ldb;
-    const bool a_there = m0 + row < p.m, b_there = n0 + row < p.n;
-    int16v_t acc;
+        for (int u = 0; u < kFewGroup; u++) {
+            const int at = min(s + u, last - 1);  // (past the end: unused)
+            g.w[u] = (uint4_t){0u, 0u, 0u, 0u};
+            if (at < whole) g.w[u] = *(const uint4_t*)(w + 64 * (int64_t)at);
+        }
+        if (real) {
 #pragma unroll
-    for (int r = 0; r < 16; r++) acc[r] = 0;
-    const int mi = 32 * (wave & 1), ni = 32 * (wave >> 1);
-    for (int64_t k0 = 0; k0 < p.k; k0 += kPlainK) {
-        const uint4_t x = load_codes16(a, k0 + 16 * piece, p.k, a_there, aligned), w = load_codes16(b, k0 + 16 * piece, p.k, b_there, aligned);
-        __syncthreads();
-        tile[0][row][piece ^ ((row >> 2) & 3)] = x;
-        tile[1][row][piece ^ ((row >> 2) & 3)] = w;
-        __syncthreads();
+            for (int u = 0; u < kFewGroup; u++) {
+                const int at = min(s + u, last - 1);
+                if (at < whole) g.x[u] = *(const uint4_t*)(x + 64 * (int64_t)at);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const auto multiply = [&](const Group& g, int s) __attribute__((always_inline)) {
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
-            const int c = 2 * s + (lane >> 5), r = lane & 31;
-            acc = mma_i8(tile[0][mi + r][c ^ (((mi + r) >> 2) & 3)], tile[1][ni + r][c ^ (((ni + r) >> 2) & 3)], acc);
+        for (int u = 0; u < kFewGroup; u++)
+            if (s + u < last) acc = mma_i8_16(g.w[u], g.x[u], acc);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (int u = 0; u < kFewGroup; u++) now.x[u] = next.x[u] = (uint4_t){0u, 0u, 0u, 0u};  // (lanes without a row keep these)
+    if (first < last) {
+        load(now, first);
+        for (int s = first; s < last; s += 2 * kFewGroup) {
+            if (s + kFewGroup < last) load(next, s + kFewGroup);
+            multiply(now, s);
+            if (s + 2 * kFewGroup < last) load(now, s + 2 * kFewGroup);
+            multiply(next, s + kFewGroup);
         }
     }
-    const int64_t col = n0 + ni + (lane & 31);
-    if (col >= p.n) return;
-    const float scale = p.b_scales ? p.b_scales[col] : 1.0f;
+    // register r: weight row 4 quarter + r, activation row lane % 16
+    sums[wave][lane] = acc;
+    __syncthreads();
+    if (wave != 0 || !real) return;
+    int4_t sum = sums[0][lane];
 #pragma unroll
-    for (int r = 0; r < 16; r++) {
-        const int64_t i = m0 + mi + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-        if (i < p.m) store_scalar(p.c, i * p.ldc + col, p.c_dtype, finished(p, acc[r], i, col, scale));
+    for (int i = 1; i < kFewWaves; i++) sum += sums[i][lane];
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int64_t column = n0 + 4 * quarter + r;
+        if (column < p.n) store_scalar(p.c, row * p.ldc + column, p.c_dtype, finished(p, sum[r], row, column, p.b_scales ? p.b_scales[column] : 1.0f));
     }
 }
 
@@ -67,12 +89,71 @@ hipattn_status checked(const hipops_matmul_i8_desc* d) {
     return HIPATTN_OK;
 }
 
+int64_t bytes_of_parts(int64_t m, int64_t n, int parts) { return parts > 1 ? parts * m * ((n + 3) / 4 * 4) * 4 : 0; }
+
+// Which kernel, and how many parts of k: the least time by a model of what was measured (us; bf16 results, weights from HBM or the last-level
+// cache), over m of 1 to 2,048 on weights of 4,096 x 4,096, 28,672 x 4,096, 4,096 x 14,336, 1,024 x 4,096, 6,144 x 4,096, 512 x 2,048, 128 x
+// 8,192 and 2,048 x 1,024: its choice is 1.3 % from the best of all choices on average, 22 % at worst (128 rows of 512 x 2,048, 9.5 for 7.8).
+// A tile costs its start and end, and for each stage of 128 bytes of k what a compute unit takes that has it alone (loads it waits
+// for) or, with more tiles than compute units, shares its time among them; the operands' bytes bound it from below.  Parts of k cost
+// the second launch and their sums' way through memory.  Where the sides cross (us): 64 x 4,096 x 4,096 tiles of 32 rows in four parts
+// 12.4, of 64 rows in four 13.1, of 128 14.0; 512 x 4,096 x 4,096 tiles of 64 18.7, of 128 21.2, of 256 33; 1,024 x 6,144 x 4,096
+// of 128 35.6, of 256 in two parts 52.7; 2,048 x 28,672 x 4,096 of 256 261, of 128 283; 16 x 4,096 x 4,096 without LDS 7.9, with 10.3;
+// 16 x 28,672 x 4,096 38.0 and 26.9; 8,192 x 6,144 x 4,096 of 256 205, of 128 236.
+struct TileCost {
+    I8Tile tile;
+    int rows, columns, most_rows;  // tiles of more rows than this are never the faster ones
+    float start, alone, shared;
+};
+constexpr TileCost kTileCosts[] = {
+    {kI8Tile32, 32, 128, 128, 3.8f, 0.33f, 0.24f},       {kI8Tile64, 64, 128, 512, 4.2f, 0.40f, 0.29f},
+    {kI8Tile128Deep, 128, 128, 1 << 30, 5.0f, 0.52f, 0.59f}, {kI8Tile128, 128, 128, 1 << 30, 6.5f, 0.65f, 0.47f},
+    {kI8Tile256, 256, 256, 1 << 30, 11.2f, 1.22f, 1.47f},
+};
+// Rows at any address, through registers (us, tiles of 32 rows / 128 rows at their best parts: 64 x 4,095 x 4,095 16.8 / -; 512 x 4,095 x 4,095
+// 39.6 / 37.1; 128 x 4,095 x 14,333 38.9 / 34.9; 100 x 2,001 x 1,001 10.4 / 17.8; 8,191 x 6,143 x 4,097 - / 391).
+constexpr TileCost kAnyCosts[] = {{kI8Any32, 32, 128, 512, 3.8f, 0.90f, 0.55f}, {kI8Any128, 128, 128, 1 << 30, 6.5f, 1.65f, 0.94f}};
+constexpr int kParts[] = {1, 2, 3, 4, 6, 8, 12, 16};
+constexpr float kUnits = 256.0f, kBytesPerUs = 7.9e6f, kSumBytesPerUs = 3.9e6f, kSecondLaunch = 2.9f;
+
+I8Plan plan_of(int64_t m, int64_t n, int64_t k, size_t workspace_bytes, bool aligned) {
+    I8Plan best{aligned ? kI8Tile32 : kI8Any32, 1};
+    float least = INFINITY;
+    const int64_t stages = (k + 127) / 128;
+    const auto consider = [&](const TileCost& t) {
+        if (m > t.most_rows) return;
+        const float tiles = (float)((m + t.rows - 1) / t.rows) * (float)((n + t.columns - 1) / t.columns);
+        for (int parts : kParts) {
+            if (parts > 1 && (stages < 2 * parts || m > 65535 || (size_t)bytes_of_parts(m, n, parts) > workspace_bytes)) break;
+            const float steps = (float)((stages + parts - 1) / parts), rounds = ceilf(tiles * parts / kUnits);
+            float us = std::max(steps * t.alone, rounds > 1.0f ? steps * rounds * t.shared : 0.0f);
+            us = t.start + std::max(us, ((float)m + (float)n) * (float)k / kBytesPerUs);
+            if (parts > 1) us += kSecondLaunch + 8.0f * parts * (float)m * (float)n / kSumBytesPerUs;
+            if (us < least) least = us, best = {t.tile, parts};
+        }
+    };
+    if (!aligned) {
+        for (const TileCost& t : kAnyCosts) consider(t);
+        return best;
+    }
+    if (m <= 16) {
+        const float steps = (float)k / 2048.0f, rounds = ceilf((float)n / 16.0f / kUnits);
+        least = 4.0f + std::max({0.405f * steps, 0.37f * rounds * steps * (1.0f + (float)m / 32.0f), (float)n * (float)k / 5.9e6f});
+        best = {kI8Few, 1};
+    }
+    for (const TileCost& t : kTileCosts) consider(t);
+    return best;
+}
+
 }  // namespace
 
 hipattn_status matmul_i8_workspace_size(const hipops_matmul_i8_desc* d, size_t* bytes) {
     if (!bytes) return fail(HIPATTN_INVALID_ARGUMENT, "matmul_i8_workspace_size: null output");
     *bytes = 0;
-    return checked(d);
+    if (const hipattn_status st = checked(d)) return st;
+    if (d->m == 0 || d->n == 0 || d->k == 0) return HIPATTN_OK;
+    *bytes = (size_t)bytes_of_parts(d->m, d->n, std::max(plan_of(d->m, d->n, d->k, SIZE_MAX, true).parts, plan_of(d->m, d->n, d->k, SIZE_MAX, false).parts));
+    return HIPATTN_OK;
 }
 
 hipattn_status matmul_i8(const hipops_matmul_i8_desc* d, const int8_t* a, const float* a_scales, const int8_t* b, const float* b_scales, const void* bias,
@@ -82,13 +163,18 @@ hipattn_status matmul_i8(const hipops_matmul_i8_desc* d, const int8_t* a, const 
     if (!c || (d->k > 0 && (!a || !b))) return fail(HIPATTN_INVALID_ARGUMENT, "matmul_i8: null pointer");
     const MatmulI8Params p{a, b, a_scales, b_scales, bias, residual, c, d->m, d->n, d->k, d->lda ? d->lda : d->k, d->ldb ? d->ldb : d->k,
                            d->ldc ? d->ldc : d->n, d->c_dtype};
-    (void)workspace;
-    (void)workspace_bytes;
-    const bool aligned = (((uintptr_t)a | (uintptr_t)b | (uintptr_t)p.lda | (uintptr_t)p.ldb) & 15) == 0;
-    const dim3 grid((unsigned)((p.n + kPlainTile - 1) / kPlainTile), (unsigned)((p.m + kPlainTile - 1) / kPlainTile));
-    if (grid.y > 65535) return fail(HIPATTN_UNSUPPORTED, "matmul_i8: %lld rows", (long long)p.m);
-    hipLaunchKernelGGL(matmul_i8_plain_kernel, grid, dim3(256), 0, stream, p, aligned ? 1 : 0);
-    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return fail(HIPATTN_HIP_ERROR, "matmul_i8: %s", hipGetErrorString(e));
+    if ((uintptr_t)workspace % 16) return fail(HIPATTN_INVALID_ARGUMENT, "matmul_i8: workspace must be 16-byte aligned");
+    // (tiles that load straight to LDS address a row from the tile's first in 32 bits)
+    const bool aligned = (((uintptr_t)a | (uintptr_t)b | (uintptr_t)p.lda | (uintptr_t)p.ldb | (uintptr_t)p.k) & 15) == 0 && p.lda <= (1 << 23) && p.ldb <= (1 << 23);
+    const I8Plan plan = plan_of(p.m, p.n, p.k, workspace ? workspace_bytes : 0, aligned);
+    hipError_t e = hipSuccess;
+    if (plan.tile == kI8Few) {
+        hipLaunchKernelGGL(matmul_i8_few_kernel, dim3((unsigned)((p.n + 15) / 16)), dim3(64 * kFewWaves), 0, stream, p);
+        e = hipGetLastError();
+    } else {
+        e = launch_matmul_i8_tiles(p, plan, workspace, stream);
+    }
+    if (e != hipSuccess) return fail(HIPATTN_HIP_ERROR, "matmul_i8: %s", hipGetErrorString(e));
     return HIPATTN_OK;
 }
 
