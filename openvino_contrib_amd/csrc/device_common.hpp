@@ -135,6 +135,18 @@ __device__ __forceinline__ float load_cache_elem(const uint8_t* row, int d, int 
     }
 }
 
+// Four values times `factor` as signed bytes: the product, rounded, plus 1.5 x 2^23 has the integer nearest to it (ties to even) in the low
+// bits of its mantissa, which two operations and the byte permutes reach where rint, clamp, conversion and shifts take seven.  The callers'
+// products lie within 127 (1 + 2^-21), so that nothing is left to clamp; infinities and NaN give some byte.
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float factor) {
+#pragma clang fp contract(off)
+    const float magic = 12582912.0f;
+    const uint32_t ia = __float_as_uint(a * factor + magic), ib = __float_as_uint(b * factor + magic);
+    const uint32_t ic = __float_as_uint(c * factor + magic), id = __float_as_uint(d * factor + magic);
+    const uint32_t lo = __builtin_amdgcn_perm(ib, ia, 0x0c0c0400u), hi = __builtin_amdgcn_perm(id, ic, 0x04000c0cu);
+    return lo | hi;
+}
+
 // ---- wavefront reductions (64 lanes) -----------------------------------------------------
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll

@@ -499,12 +499,10 @@ __device__ __forceinline__ void block_vector(const RopeAppendParams& p, const Bl
         for (int i = 0; i < kAhead; i++) {
             const int r = n0 + i * l.rows + l.row;
             if (!l.active || r >= n) continue;
-            int q[2][8];
-#pragma unroll
-            for (int e = 0; e < 16; e++) q[e >> 3][e & 7] = code_of(x[i][e], inverse);
+            const float* const v = x[i];
             int8_t* const dst = codes + (int64_t)(b.r0 + r) * p.head_dim;
-            *(uint2_t*)(dst + u.d0) = pack_bytes(q[0]);
-            *(uint2_t*)(dst + u.d1) = pack_bytes(q[1]);
+            *(uint2_t*)(dst + u.d0) = (uint2_t){codes4(v[0], v[1], v[2], v[3], inverse), codes4(v[4], v[5], v[6], v[7], inverse)};
+            *(uint2_t*)(dst + u.d1) = (uint2_t){codes4(v[8], v[9], v[10], v[11], inverse), codes4(v[12], v[13], v[14], v[15], inverse)};
         }
     }
     if (lane == 0) *scales = scale;
