@@ -91,30 +91,32 @@ hipattn_status checked(const hipops_matmul_i8_desc* d) {
 
 int64_t bytes_of_parts(int64_t m, int64_t n, int parts) { return parts > 1 ? parts * m * ((n + 3) / 4 * 4) * 4 : 0; }
 
-// Which kernel, and how many parts of k: the least time by a model of what was measured (us; bf16 results, weights from HBM or the last-level
-// cache), over m of 1 to 2,048 on weights of 4,096 x 4,096, 28,672 x 4,096, 4,096 x 14,336, 1,024 x 4,096, 6,144 x 4,096, 512 x 2,048, 128 x
-// 8,192 and 2,048 x 1,024: its choice is 1.3 % from the best of all choices on average, 22 % at worst (128 rows of 512 x 2,048, 9.5 for 7.8).
-// A tile costs its start and end, and for each stage of 128 bytes of k what a compute unit takes that has it alone (loads it waits
-// for) or, with more tiles than compute units, shares its time among them; the operands' bytes bound it from below.  Parts of k cost
-// the second launch and their sums' way through memory.  Where the sides cross (us): 64 x 4,096 x 4,096 tiles of 32 rows in four parts
-// 12.4, of 64 rows in four 13.1, of 128 14.0; 512 x 4,096 x 4,096 tiles of 64 18.7, of 128 21.2, of 256 33; 1,024 x 6,144 x 4,096
-// of 128 35.6, of 256 in two parts 52.7; 2,048 x 28,672 x 4,096 of 256 261, of 128 283; 16 x 4,096 x 4,096 without LDS 7.9, with 10.3;
-// 16 x 28,672 x 4,096 38.0 and 26.9; 8,192 x 6,144 x 4,096 of 256 205, of 128 236.
+// Which kernel, and how many parts of k: the least time by a model of what was measured (us; bf16 results, three sets of operands in
+// turn), over 160 sizes: m of 1 to 8,192 on weights of 4,096 x 4,096, 28,672 x 4,096, 11,008 x 4,096, 4,096 x 14,336, 2,560 x 10,240, 1,024 x
+// 4,096, 6,144 x 4,096 and 2,048, 512 x 2,048, 320 and 2,048 x 1,024, 128 x 8,192.  Its choice is 0.9 % from the best of all choices on
+// average, 22 % at worst (128 rows of 512 x 2,048: 9.5 for 7.8).
+// A tile costs its start and end, and for each stage of 128 bytes of k the largest of: what a compute unit takes that has one tile
+// (`alone`: the loads it waits for); with more tiles than compute units, what the fullest takes (`together`) and the whole device
+// (`through`: power and the caches).  The operands' bytes bound it from below.  Parts of k cost the second launch and their sums' way
+// through memory.  Where the sides cross (us): 64 x 4,096 x 4,096 tiles of 32 rows in four parts 12.4, of 64 in four 13.1, of 128 14.0;
+// 512 x 4,096 x 4,096 tiles of 64 18.7, of 128 with a deep ring 21.2, of 128 26.8, of 256 33; 1,024 x 6,144 x 4,096 of 128 35.6, deep 43.0, of
+// 256 52.7; 1,111 x 4,096 x 14,336 of 128 90, of 256 in three parts 91; 3,000 x 4,096 x 14,336 of 256 190, of 128 209; 8,192 x 6,144 x 4,096
+// of 256 205, of 128 236; 16 x 4,096 x 4,096 without LDS 7.9, with 10.3; 16 x 28,672 x 4,096 38.0 and 26.9.
 struct TileCost {
     I8Tile tile;
     int rows, columns, most_rows;  // tiles of more rows than this are never the faster ones
-    float start, alone, shared;
+    float start, alone, together, through;
 };
 constexpr TileCost kTileCosts[] = {
-    {kI8Tile32, 32, 128, 128, 3.8f, 0.33f, 0.24f},       {kI8Tile64, 64, 128, 512, 4.2f, 0.40f, 0.29f},
-    {kI8Tile128Deep, 128, 128, 1 << 30, 5.0f, 0.52f, 0.59f}, {kI8Tile128, 128, 128, 1 << 30, 6.5f, 0.65f, 0.47f},
-    {kI8Tile256, 256, 256, 1 << 30, 11.2f, 1.22f, 1.47f},
+    {kI8Tile32, 32, 128, 128, 3.7f, 0.41f, 0.32f, 0.28f},           {kI8Tile64, 64, 128, 1600, 4.1f, 0.43f, 0.29f, 0.46f},
+    {kI8Tile128Deep, 128, 128, 1 << 30, 5.1f, 0.52f, 0.66f, 0.60f}, {kI8Tile128, 128, 128, 1 << 30, 7.0f, 0.67f, 0.37f, 0.59f},
+    {kI8Tile256, 256, 256, 1 << 30, 11.7f, 1.39f, 1.53f, 1.91f},
 };
 // Rows at any address, through registers (us, tiles of 32 rows / 128 rows at their best parts: 64 x 4,095 x 4,095 16.8 / -; 512 x 4,095 x 4,095
 // 39.6 / 37.1; 128 x 4,095 x 14,333 38.9 / 34.9; 100 x 2,001 x 1,001 10.4 / 17.8; 8,191 x 6,143 x 4,097 - / 391).
-constexpr TileCost kAnyCosts[] = {{kI8Any32, 32, 128, 512, 3.8f, 0.90f, 0.55f}, {kI8Any128, 128, 128, 1 << 30, 6.5f, 1.65f, 0.94f}};
+constexpr TileCost kAnyCosts[] = {{kI8Any32, 32, 128, 512, 3.8f, 0.90f, 0.55f, 0.55f}, {kI8Any128, 128, 128, 1 << 30, 6.5f, 1.65f, 0.94f, 0.94f}};
 constexpr int kParts[] = {1, 2, 3, 4, 6, 8, 12, 16};
-constexpr float kUnits = 256.0f, kBytesPerUs = 7.9e6f, kSumBytesPerUs = 3.9e6f, kSecondLaunch = 2.9f;
+constexpr float kUnits = 256.0f, kBytesPerUs = 5.95e6f, kSumBytesPerUs = 3.8e6f, kSecondLaunch = 2.7f;
 
 I8Plan plan_of(int64_t m, int64_t n, int64_t k, size_t workspace_bytes, bool aligned) {
     I8Plan best{aligned ? kI8Tile32 : kI8Any32, 1};
@@ -125,9 +127,9 @@ I8Plan plan_of(int64_t m, int64_t n, int64_t k, size_t workspace_bytes, bool ali
         const float tiles = (float)((m + t.rows - 1) / t.rows) * (float)((n + t.columns - 1) / t.columns);
         for (int parts : kParts) {
             if (parts > 1 && (stages < 2 * parts || m > 65535 || (size_t)bytes_of_parts(m, n, parts) > workspace_bytes)) break;
-            const float steps = (float)((stages + parts - 1) / parts), rounds = ceilf(tiles * parts / kUnits);
-            float us = std::max(steps * t.alone, rounds > 1.0f ? steps * rounds * t.shared : 0.0f);
-            us = t.start + std::max(us, ((float)m + (float)n) * (float)k / kBytesPerUs);
+            const float steps = (float)((stages + parts - 1) / parts), each = tiles * parts / kUnits;
+            const float stage = std::max({t.alone, each > 1.0f ? ceilf(each) * t.together : 0.0f, each * t.through});
+            float us = t.start + std::max(steps * stage, ((float)m + (float)n) * (float)k / kBytesPerUs);
             if (parts > 1) us += kSecondLaunch + 8.0f * parts * (float)m * (float)n / kSumBytesPerUs;
             if (us < least) least = us, best = {t.tile, parts};
         }
@@ -138,7 +140,7 @@ I8Plan plan_of(int64_t m, int64_t n, int64_t k, size_t workspace_bytes, bool ali
     }
     if (m <= 16) {
         const float steps = (float)k / 2048.0f, rounds = ceilf((float)n / 16.0f / kUnits);
-        least = 4.0f + std::max({0.405f * steps, 0.37f * rounds * steps * (1.0f + (float)m / 32.0f), (float)n * (float)k / 5.9e6f});
+        least = 3.9f + std::max({0.41f * steps, 0.365f * rounds * steps * (1.0f + (float)m / 32.0f), (float)n * (float)k / 4.7e6f});
         best = {kI8Few, 1};
     }
     for (const TileCost& t : kTileCosts) consider(t);
