@@ -194,7 +194,7 @@ struct PagedParams {
                           // chunked-prefill kernel too (HIPATTN_PA_ANY_LENGTHS); without it such a batch is
                           // planned per token and every token is a decode row
     int no_side_stream;   // mixed batches run one kernel after the other on the caller's stream
-    // u8 caches, nullptr or: what the writer left of the new rows of sequences without cached tokens and with kShadowTokens or more, as a chunk
+    // u8 and i8 caches, nullptr or: what the writer (i8: the prologue) left of the new rows of sequences without cached tokens and with kShadowTokens or more, as a chunk
     // kernel finds them in the cache but in fp16 -- [blocks, num_heads_kv, block_size, head_dim], a sequence's blocks from shadow_block()
     // on, and a block table that counts from there (-1: the cache's table names no block, whose rows are zeros here)
     uint16_t* shadow_k;

@@ -17,7 +17,7 @@ from openvino_contrib_amd import workloads as W
 pytestmark = pytest.mark.gpu
 
 
-def run(hip, b, q_dtype=F16, out_dtype=None, window=0, flags=0, scale=0.0, sinks=None, alibi=None, new_rows=None, bound_len=None):
+def run(hip, b, q_dtype=F16, out_dtype=None, window=0, flags=0, scale=0.0, sinks=None, alibi=None, new_rows=None, bound_len=None, small_workspace=False):
     out_dtype = q_dtype if out_dtype is None else out_dtype
     dev = R.Device(hip, b)
     T = b.tokens
@@ -30,7 +30,10 @@ def run(hip, b, q_dtype=F16, out_dtype=None, window=0, flags=0, scale=0.0, sinks
     keep = [up(x) if x is not None else None for x in (sinks, alibi)]
     pa = hip.PaDesc(q_dtype, F16, I8, out_dtype, b.Hq, b.Hkv, b.D, b.bs, b.blocks, T, len(b.seqs), b.longest if bound_len is None else bound_len,
                     window, scale, skip | flags, 0, keep[1].ptr if keep[1] else None, keep[0].ptr if keep[0] else None)
+    if small_workspace:  # (what a bound on the contexts leaves out: room for the new prompts in fp16)
+        pa.max_context_len = 64
     ws = hip.DeviceBuffer(max(16, hip.paged_attention_workspace_size(pa)))
+    pa.max_context_len = b.longest if bound_len is None else bound_len
     ws.fill(0xA5)
     k, v = (up(x) for x in new_rows) if new_rows is not None else (None, None)
     hip.paged_attention_i8(pa, up(q_st), k, v, *dev.caches, *dev.scales, *dev.index, out, ws)
@@ -188,6 +191,24 @@ def test_long_context_and_many_rows(hip):
     check(hip, b, bound_of(True, F16, F32, True), out_dtype=F32, bound_len=0)
     b = R.Batch(13, [(i * 7 % 90, 1) for i in range(300)], 4, 1, 128, 32)
     check(hip, b, bound_of(True, F16, F32, False), out_dtype=F32)
+
+
+@pytest.mark.parametrize("bs", [16, 32, 64])
+def test_new_prompts_are_expanded_once(hip, bs):
+    """Prompts long enough for a copy of their rows in fp16 beside short ones, others behind cached tokens and decode rows, with and without
+    room for the copy; entries without a block among the prompts', scales that are not numbers in blocks that nobody uses."""
+    for seqs in ([(0, 400), (0, 383), (0, 700), (100, 450), (0, 1), (900, 1), (0, 384)], [(0, 1000)], [(0, 500), (0, 0), (3, 2)]):
+        for edit in (False, True):
+            b = R.Batch(14, seqs, 4, 2, 128, bs)
+            if edit:
+                b.table[2::7] = -1
+                b.table[4::9] = b.blocks
+            used = set(int(x) for x in b.table)
+            for i in set(range(b.blocks)) - used:
+                b.scales[:, i] = np.nan
+            for small in (False, True):
+                check(hip, b, bound_of(True, F16, F32, True), out_dtype=F32, small_workspace=small)
+            check(hip, b, bound_of(True, BF16, BF16, True), q_dtype=BF16, window=333)
 
 
 def test_refusals(hip):
