@@ -200,6 +200,10 @@ struct PagedParams {
     uint16_t* shadow_k;
     uint16_t* shadow_v;
     int32_t* shadow_table;
+    // i8 caches: sequences of kShadowTokens new tokens or more, cached tokens included; a sequence's blocks from shadow_base[s] on (-1: none),
+    // beginning with the first that its window leaves; shadow_capacity blocks in all
+    int32_t* shadow_base;
+    int shadow_capacity;
     int tiles_only;       // (flash_small.hip) tile_prefix counts single-token sequences too: there are no decode rows
     int lone_tile;        // (paged_mixed.hip) one sequence, which gets query tiles also if it is a single token: no decode rows, no merge
 };

@@ -79,7 +79,7 @@ __device__ __forceinline__ void plan_block(const PagedParams& p) {
         // proportion to its work, so that both end together.
         const bool u8 = eight_bit(p.cache_dtype);
         const float decode_us = (float)total_blk * p.num_heads_kv * (u8 ? 8704.0f / 24000.0f : 16384.0f / 33000.0f) * p.overlap_share;
-        const float prefill_us = total_keys * p.num_heads_q * (u8 ? 1.4f : 1.1f);
+        const float prefill_us = total_keys * p.num_heads_q * (p.shadow_base != nullptr ? 1.2f : u8 ? 1.4f : 1.1f);  // (i8: expanded once)
         const int cus = p.num_waves >> 3;
         int mine = (int)ceilf(cus * decode_us / fmaxf(decode_us + prefill_us, 1.0f));
         mine = max(1, min(mine, cus));
@@ -104,39 +104,78 @@ __device__ __forceinline__ void plan_block(const PagedParams& p) {
     }
 }
 
-// The rows of an i8 cache's new prompts in fp16 (PagedParams::shadow_k), for the chunk kernel, which works through each of them once per
-// 128 query rows and pair of heads and would turn codes into numbers every time, in the phase that bounds it.  A wavefront to a (block,
-// kv head, K or V).  Measured (us a step, 32 heads on 8, without -> with): six
-// prompts of 100 to 3,000 tokens 190 -> 147, two of 3,000 230 -> 179, one of 1,000 47.5 -> 39.6, eight of 400 56.5 -> 51.1.
-__device__ __forceinline__ void expand_block_i8(const PagedParams& p, int64_t wv, int lane) {
-    const int Hkv = p.num_heads_kv / p.kv_share, per_block = 2 * Hkv;
-    const int64_t index = wv / per_block;
-    const int which = (int)(wv % per_block), h = which >> 1;
-    // the last sequence whose blocks begin at or before this one, 64 of them a step
-    int lo = 0, hi = p.num_seqs;
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 63) / 64, at = lo + lane * step;
-        const bool ok = at < hi && shadow_block(p.subsequence_begins[at], at, p.block_size) <= index;
-        const int k = max(__builtin_popcountll(__builtin_amdgcn_ballot_w64(ok)) - 1, 0);
-        lo = lo + k * step;
-        hi = min(hi, lo + step);
+// The rows that the chunks of an i8 cache attend, in fp16 (PagedParams::shadow_k), for the chunk kernel, which works through each of them
+// once per 128 query rows and pair of heads and would turn codes into numbers every time, in the phase that bounds it.  Sequences of
+// kShadowTokens new tokens or more get it, cached tokens included, from the first block that the window leaves; as many as p.shadow_capacity
+// blocks hold, in their order.  Four workgroups to a block, K and V and half the kv heads each; the first one also leaves where each
+// sequence's begin.
+// Measured (us a step, 32 heads on 8, without -> with): six prompts of 100 to 3,000 tokens 189 -> 148, two of 3,000 228 -> 182, one of 1,000
+// 47.5 -> 39.8, eight of 400 55.9 -> 52.7; eight chunks of 512 behind 4,096 tokens (64 heads) 485 -> 389, with a window of that and 120 decode
+// rows 581 -> 513, one of 400 behind 4,096 160 -> 112.
+__device__ __forceinline__ void expand_blocks_i8(const PagedParams& p, int workgroup) {
+    const int lane = threadIdx.x & 63, index = workgroup >> 2, part = workgroup & 3;
+    const bool leaves = workgroup == 0 && threadIdx.x < 64;
+    int carry = 0, owner = -1, base = 0, first = 0;
+    for (int s0 = 0; s0 < p.num_seqs; s0 += 64) {
+        const int s = s0 + lane;
+        int n = 0, f = 0;
+        if (s < p.num_seqs) {
+            const int begin = p.subsequence_begins[s], end = p.subsequence_begins[s + 1], past = p.past_lens[s];
+            const int entries = p.block_indices_begins[s + 1] - p.block_indices_begins[s];
+            if (begin >= 0 && end <= p.num_tokens && end - begin >= kShadowTokens && past >= 0) {
+                // (whole 64-key tiles, as the chunk kernel visits them)
+                f = p.sliding_window > 0 ? (max(0, past - p.sliding_window + 1) & ~63) / p.block_size : 0;
+                n = max(0, min(entries, (past + (end - begin) + p.block_size - 1) / p.block_size) - f);
+            }
+        }
+        int scan = n;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int up = __shfl_up(scan, d, 64);
+            if (lane >= d) scan += up;
+        }
+        const int at = carry + scan - n;
+        const bool fits = n > 0 && at + n <= p.shadow_capacity;
+        if (leaves && s < p.num_seqs) p.shadow_base[s] = fits ? at : -1;
+        const uint64_t mine = __builtin_amdgcn_ballot_w64(fits && index >= at && index < at + n);
+        if (mine) {
+            const int l = __builtin_ctzll(mine);
+            owner = s0 + l;
+            base = __shfl(at, l, 64);
+            first = __shfl(f, l, 64);
+            if (!leaves) break;
+        }
+        carry += __shfl(scan, 63, 64);
     }
-    const int begin = p.subsequence_begins[lo], end = p.subsequence_begins[lo + 1], table = p.block_indices_begins[lo];
-    const int64_t lb = index - shadow_block(begin, lo, p.block_size);
-    const int entries = min(p.block_indices_begins[lo + 1] - table, (end - begin + p.block_size - 1) / p.block_size);
-    if (p.past_lens[lo] != 0 || begin < 0 || end > p.num_tokens || end - begin < kShadowTokens || lb < 0 || lb >= entries) return;
-    const int pb = p.block_indices[table + lb];
+    if (owner < 0) return;
+    const int pb = p.block_indices[p.block_indices_begins[owner] + first + (index - base)];
     const bool there = pb >= 0 && pb < p.num_blocks;
-    if (which == 0 && lane == 0) p.shadow_table[index] = there ? (int)lb : -1;
-    const int64_t bytes = (int64_t)p.block_size * 128, to = (index * Hkv + h) * bytes;
-    const uint8_t* const codes = ((which & 1) ? p.value_cache : p.key_cache) + ((int64_t)(there ? pb : 0) * Hkv + h) * bytes;
-    uint16_t* const out = ((which & 1) ? p.shadow_v : p.shadow_k) + to;
-    const float scale = there ? ((which & 1) ? p.value_scales : p.key_scales)[(int64_t)pb * Hkv + h] : 0.0f;
-    const SplitScale s = split_scale(fabsf(scale) < INFINITY ? scale : 0.0f);
-    for (int64_t i = 16 * lane; i < bytes; i += 16 * 64) {
-        const uint4_t w = *(const uint4_t*)(codes + i);
-        *(uint4_t*)(out + i) = dequant_codes8((uint2_t){w[0], w[1]}, s);
-        *(uint4_t*)(out + i + 8) = dequant_codes8((uint2_t){w[2], w[3]}, s);
+    if (part == 0 && threadIdx.x == 0) p.shadow_table[index] = there ? index - base : -1;
+    const int Hkv = p.num_heads_kv / p.kv_share;
+    const int pieces = p.block_size * 8, shift = __builtin_ctz(pieces);  // sixteen codes each, of a head's rows
+    const bool value = part & 1;
+    const uint8_t* const codes = (value ? p.value_cache : p.key_cache) + (int64_t)(there ? pb : 0) * Hkv * pieces * 16;
+    uint16_t* const out = (value ? p.shadow_v : p.shadow_k) + (int64_t)index * Hkv * pieces * 16;
+    const float* const scales = (value ? p.value_scales : p.key_scales) + (int64_t)(there ? pb : 0) * Hkv;
+    const int middle = (Hkv * pieces / 2 + 255) & ~255, last = part & 2 ? Hkv * pieces : min(middle, Hkv * pieces);
+    constexpr int kAtOnce = 4;
+    for (int i0 = (part & 2 ? middle : 0) + (int)threadIdx.x; i0 < last; i0 += 256 * kAtOnce) {
+        uint4_t w[kAtOnce];
+        float scale[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; u++) {
+            const int i = min(i0 + 256 * u, last - 1);
+            w[u] = *(const uint4_t*)(codes + (int64_t)i * 16);
+            scale[u] = there ? scales[i >> shift] : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < kAtOnce; u++) {
+            const int i = i0 + 256 * u;
+            if (i >= last) break;
+            const SplitScale sc = split_scale(fabsf(scale[u]) < INFINITY ? scale[u] : 0.0f);
+            *(uint4_t*)(out + (int64_t)i * 16) = dequant_codes8((uint2_t){w[u][0], w[u][1]}, sc);
+            *(uint4_t*)(out + (int64_t)i * 16 + 8) = dequant_codes8((uint2_t){w[u][2], w[u][3]}, sc);
+        }
     }
 }
 
@@ -146,8 +185,8 @@ __device__ __forceinline__ void expand_block_i8(const PagedParams& p, int64_t wv
 __global__ __launch_bounds__(256) void paged_prologue_kernel(KvWriteParams wp, PagedParams p, int write_blocks) {
     if ((int)blockIdx.x < write_blocks) {
         const int64_t wv = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-        if (p.cache_dtype == HIPATTN_I8)  // (written already; these are the new prompts' copies)
-            expand_block_i8(p, wv, threadIdx.x & 63);
+        if (p.cache_dtype == HIPATTN_I8)  // (written already)
+            expand_blocks_i8(p, (int)blockIdx.x);
         else if (wp.head_dim <= 128)  // (elements of a row per lane: two up to head size 128, four up to 256)
             kv_cache_write_wave<2>(wp, wv, threadIdx.x & 63);
         else
@@ -980,10 +1019,25 @@ size_t paged_fast_workspace_bytes(const PagedParams& p) {
 // heads) 283 -> 274.  Up to 256 MiB (65,536 tokens of 8 heads).
 static int64_t shadow_blocks(const PagedParams& p) { return (int64_t)(p.num_tokens / p.block_size) + p.num_seqs + 1; }
 
+// i8 caches: blocks that the batch's sequences of kShadowTokens new tokens or more can attend; their lengths stay on the device, which takes
+// as many sequences as fit.  (Every workgroup of the expansion looks through the sequences: not in batches of very many.)
+constexpr int kShadowSeqs = 1024;
+static size_t shadow_block_bytes(const PagedParams& p) { return 2 * (size_t)(p.num_heads_kv / p.kv_share) * p.block_size * 128 * sizeof(uint16_t); }
+static int64_t shadow_bound_i8(const PagedParams& p) {
+    const int64_t most = std::min<int64_t>(p.num_seqs, p.num_tokens / kShadowTokens);
+    int64_t context = p.max_context_len > 0 ? p.max_context_len : (int64_t)1 << 31;
+    if (p.sliding_window > 0) context = std::min<int64_t>(context, (int64_t)p.sliding_window + p.num_tokens + 64);
+    return std::min<int64_t>(most * ((context + p.block_size - 1) / p.block_size + 1), p.num_blocks);
+}
+
 size_t paged_shadow_bytes(const PagedParams& p) {
     if (!eight_bit(p.cache_dtype) || p.head_dim != 128 || !overlap_wanted(p) || !paged_mixed_supported(p)) return 0;
     if (p.num_tokens < kShadowTokens || (p.max_context_len > 0 && p.max_context_len < kShadowTokens)) return 0;
     const int64_t kv_heads = p.num_heads_kv / p.kv_share;
+    if (p.cache_dtype == HIPATTN_I8) {
+        const int64_t blocks = std::min(shadow_bound_i8(p), (int64_t)((size_t)256 << 20) / (int64_t)shadow_block_bytes(p));
+        return p.num_seqs > kShadowSeqs || blocks <= 0 ? 0 : 256 + align_up((size_t)p.num_seqs * sizeof(int32_t), 256) + (size_t)blocks * (shadow_block_bytes(p) + sizeof(int32_t));
+    }
     const size_t rows = (size_t)(shadow_blocks(p) * kv_heads * p.block_size) * 128 * sizeof(uint16_t);
     return rows > (size_t)128 << 20 ? 0 : 256 + 2 * rows + align_up((size_t)shadow_blocks(p) * sizeof(int32_t), 256);
 }
@@ -1041,7 +1095,23 @@ void paged_fast_plan(PagedParams& p, void* workspace, size_t workspace_bytes) {
     w += align_up(slots * G * 2 * sizeof(float), 256);
     p.part_flag = (uint64_t*)w;
     w += align_up(slots * sizeof(uint64_t), 256);
-    if (shadow > 0 && (size_t)(w - (uint8_t*)workspace) + shadow <= workspace_bytes) {
+    const size_t used = (size_t)(w - (uint8_t*)workspace);
+    if (p.cache_dtype == HIPATTN_I8) {
+        // (what the caller has: a call without a bound on its contexts would ask for more than the one that sized the workspace)
+        const size_t head = 256 + align_up((size_t)p.num_seqs * sizeof(int32_t), 256);
+        if (shadow > 0 && workspace_bytes > used + head) {
+            p.shadow_capacity = (int)(std::min(shadow, workspace_bytes - used) - std::min(shadow, head)) / (int)(shadow_block_bytes(p) + sizeof(int32_t));
+        }
+        if (p.shadow_capacity > 0) {
+            w += (256 - (uintptr_t)w % 256) % 256;
+            const size_t rows = (size_t)p.shadow_capacity * shadow_block_bytes(p) / 2;
+            p.shadow_base = (int32_t*)w;
+            w += align_up((size_t)p.num_seqs * sizeof(int32_t), 256);
+            p.shadow_k = (uint16_t*)w;
+            p.shadow_v = (uint16_t*)(w + rows);
+            p.shadow_table = (int32_t*)(w + 2 * rows);
+        }
+    } else if (shadow > 0 && used + shadow <= workspace_bytes) {
         w += (256 - (uintptr_t)w % 256) % 256;
         const size_t rows = (size_t)(shadow_blocks(p) * (p.num_heads_kv / p.kv_share) * p.block_size) * 128;
         p.shadow_k = (uint16_t*)w;
@@ -1296,7 +1366,7 @@ hipError_t launch_paged_fast(const PagedParams& params, const KvWriteParams* wri
     if (wp.vector_rows)
         wp.shadow_k = p.shadow_k, wp.shadow_v = p.shadow_v, wp.shadow_table = p.shadow_table;
     else if (p.cache_dtype == HIPATTN_I8 && p.shadow_table != nullptr)
-        write_blocks = (int)((shadow_blocks(p) * 2 * (p.num_heads_kv / p.kv_share) + 3) / 4);
+        write_blocks = 4 * p.shadow_capacity;
     else
         p.shadow_table = nullptr;  // (nobody to fill it)
     hipError_t e = hipSuccess;

@@ -197,7 +197,7 @@ def test_long_context_and_many_rows(hip):
 def test_new_prompts_are_expanded_once(hip, bs):
     """Prompts long enough for a copy of their rows in fp16 beside short ones, others behind cached tokens and decode rows, with and without
     room for the copy; entries without a block among the prompts', scales that are not numbers in blocks that nobody uses."""
-    for seqs in ([(0, 400), (0, 383), (0, 700), (100, 450), (0, 1), (900, 1), (0, 384)], [(0, 1000)], [(0, 500), (0, 0), (3, 2)]):
+    for seqs in ([(0, 400), (0, 383), (0, 700), (100, 450), (0, 1), (900, 1), (0, 384)], [(0, 1000)], [(0, 500), (0, 0), (3, 2)], [(1000, 390), (77, 2), (2100, 600)]):
         for edit in (False, True):
             b = R.Batch(14, seqs, 4, 2, 128, bs)
             if edit:
@@ -209,6 +209,7 @@ def test_new_prompts_are_expanded_once(hip, bs):
             for small in (False, True):
                 check(hip, b, bound_of(True, F16, F32, True), out_dtype=F32, small_workspace=small)
             check(hip, b, bound_of(True, BF16, BF16, True), q_dtype=BF16, window=333)
+            check(hip, b, bound_of(True, F16, F32, True), out_dtype=F32, window=1500, bound_len=0)
 
 
 def test_refusals(hip):
