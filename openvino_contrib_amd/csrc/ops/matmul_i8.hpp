@@ -93,6 +93,7 @@ struct I8Grid {
     int tiles_m, tiles_n, tiles, parts;
     int group_rows;  // tiles of m that are gone through before the next tile of n
     int xcd_run;     // tiles that an XCD takes
+    int rotate;      // tiles begin at different stages of k
     int* sums;       // null, or [parts][m][sums_stride]
     int64_t sums_stride;
 };
