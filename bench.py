@@ -19,7 +19,7 @@ sample of the same workload.  `plugin_ms_per_step` of the headline workload is t
 the plugin layer's InferRequest::infer with device-resident tensors.  Everything that is not one of
 the four configurations runs only when asked for: --workload layer (the operators of libhipops.so),
 shapes (other cache shapes), decoder (a decoder layer through the plugin), scores (the operator's
-second output), masked (config 2's shape with the causality as an attention mask).
+second output), masked (config 2's shape with the causality as an attention mask), int8 (the decoder layer in 8 bits).
 """
 import argparse
 import json
@@ -852,6 +852,67 @@ def bench_decoder_layer(hip, steps, warmup):
     return res
 
 
+def bench_int8_layer(hip, steps, warmup):
+    """The decoder layer of bench_decoder_layer in 8 bits (weights, activations ahead of each product, KV cache) on config 3's batch: the ten
+    calls of int8_layer.py, eager and as one recorded graph.  The step has to read the weights and the batch's cache once."""
+    import ctypes
+    import numpy as np
+    from openvino_contrib_amd import int8_layer as L
+    from openvino_contrib_amd import workloads as W
+
+    hidden, Hq, Hkv, D, ffn, bs, S = 4096, 32, 8, 128, 14336, 32, 64
+    rng = np.random.Generator(np.random.PCG64(1003))
+    ctx = rng.integers(512, 8193, size=S)
+    blocks_of = -(-ctx // bs)
+    blocks = int(blocks_of.sum()) + 3
+    up = hip.DeviceBuffer.from_numpy
+
+    def weights(n, k):
+        return L.Weights(rng.integers(-127, 128, (n, k), dtype=np.int8), np.full(n, 1 / (73 * np.sqrt(k)), np.float32))
+
+    half = np.arange(0, D, 2, dtype=np.float64) / D
+    ang = np.arange(int(ctx.max()), dtype=np.float64)[:, None] * (10000.0 ** -half)[None, :]
+    table = [up(np.concatenate([f(ang), f(ang)], 1).astype(np.float32)) for f in (np.cos, np.sin)]
+    gamma = [up(W.to_storage(1.0 + 0.1 * rng.standard_normal(hidden).astype(np.float32), W.BF16)[0]) for _ in range(2)]
+    layer = L.DecoderLayerI8(weights((Hq + 2 * Hkv) * D, hidden), weights(hidden, Hq * D), weights(2 * ffn, hidden), weights(hidden, ffn), *gamma, *table,
+                             int(ctx.max()), Hq, Hkv, D)
+    layer.prepare(S, S, blocks, bs, int(ctx.max()))
+    some = rng.integers(-127, 128, (2048, Hkv, bs, D), dtype=np.int8)  # (repeated over the pool; the block table scatters them)
+    caches = [up(np.concatenate([some] * (-(-blocks // 2048)))[:blocks]) for _ in range(2)]
+    scales = [up(np.full((blocks, Hkv), 4 / 127, np.float32)) for _ in range(2)]
+    begins = np.concatenate([[0], np.cumsum(blocks_of)]).astype(np.int32)
+    index = [up(a) for a in ((ctx - 1).astype(np.int32), np.arange(S + 1, dtype=np.int32), rng.permutation(blocks)[:begins[-1]].astype(np.int32), begins)]
+    x = up(W.to_storage(rng.standard_normal((S, hidden)).astype(np.float32), W.BF16)[0])
+    out, stream = hip.DeviceBuffer(S * hidden * 2), hip.Stream()
+    step = lambda: layer.step(x, out, *caches, *scales, index, stream)
+    for _ in range(max(warmup, 30)):
+        step()
+    graph = ctypes.c_void_p()
+    hip.check(hip.lib().hipattn_stream_begin_capture(stream.handle))
+    step()
+    hip.check(hip.lib().hipattn_stream_end_capture(stream.handle, ctypes.byref(graph)))
+    ms = {}
+    for name, run in (("eager", step), ("graph", lambda: hip.check(hip.lib().hipattn_graph_launch(graph, stream.handle)))):
+        for _ in range(10):
+            run()
+        stream.synchronize()
+        before, after = hip.Event(), hip.Event()
+        before.record(stream)
+        for _ in range(steps):
+            run()
+        after.record(stream)
+        after.synchronize()
+        ms[name] = before.elapsed_ms(after) / steps
+    hip.check(hip.lib().hipattn_graph_destroy(graph))
+    weight_bytes = hidden * (Hq + 2 * Hkv) * D + hidden * Hq * D + 3 * hidden * ffn
+    kv_bytes = int(2 * Hkv * (ctx.sum() * D + 4 * blocks_of.sum()))
+    achieved = (weight_bytes + kv_bytes) / (ms["graph"] * 1e-3) / 1e9
+    return {"workload": "decoder layer (hidden 4096, 32/8 heads of 128, MLP 14336) in 8 bits on config3's decode batch: ten calls of the C ABI",
+            "ms_per_step": ms["graph"], "eager_ms_per_step": ms["eager"], "weight_bytes": weight_bytes, "kv_bytes": kv_bytes,
+            "roofline": {"bound": "hbm", "achieved": achieved, "peak": HBM_PEAK_GBS, "unit": "GB/s", "frac": achieved / HBM_PEAK_GBS, "traffic": None,
+                         "note": "the recorded step over the bytes it must read (weights + cached codes)"}}
+
+
 def _r(x, digits=5):
     """Floats to `digits` significant digits: the compact line is for a reader, the detail file keeps everything."""
     return float("%.*g" % (digits, x)) if isinstance(x, float) else x
@@ -885,7 +946,7 @@ def main():
     ap.add_argument("--gpus", type=int, default=1)
     ap.add_argument("--steps", type=int, default=200)
     ap.add_argument("--warmup", type=int, default=20)
-    ap.add_argument("--workload", default="c3", choices=["c2", "c3", "c4", "c5", "c5u8", "layer", "shapes", "mqa", "decoder", "scores", "masked", "copy", "mfma", "stream", "writer"],
+    ap.add_argument("--workload", default="c3", choices=["c2", "c3", "c4", "c5", "c5u8", "layer", "shapes", "mqa", "decoder", "scores", "masked", "copy", "mfma", "stream", "writer", "int8"],
                     help="copy = plain 1 GiB device copy and fill, the yardstick for hardware byte counters; "
                          "mfma = register-fed bf16 MFMAs only, the yardstick for the MFMA-bound kernels; "
                          "stream = a plain reader on a share of the compute units, alone and beside config 5's chunks; "
@@ -948,6 +1009,11 @@ def main():
     if args.workload == "decoder":
         print(json.dumps({"workload": "decoder", "steps": args.steps, "warmup": args.warmup,
                           "workloads": {"decoder_layer": bench_decoder_layer(hip, args.steps, args.warmup)}}))
+        return
+
+    if args.workload == "int8":
+        print(json.dumps({"workload": "int8", "steps": args.steps, "warmup": args.warmup,
+                          "workloads": {"decoder_layer_int8": bench_int8_layer(hip, args.steps, args.warmup)}}))
         return
 
     if args.workload == "mqa":
