@@ -979,6 +979,9 @@ static int choose_num_waves(const PagedParams& p, bool overlap) {
     // (u8 at head size 64 has the most arithmetic per byte of all: every resident wavefront, 0.59 against
     // 0.48 of HBM peak with six per compute unit on the 128-sequence u8 batch)
     if (p.head_dim > 128) return resident;  // half as many bytes in flight per wavefront: twice the wavefronts
+    // (i8 below head size 128, padded ones among them: 64 sequences of 512 to 8,192 tokens at head size 64 68 us with eight, 76 with six;
+    // at 80 89 and 103; at 128 with six 117, with eight 123, with four 118 and 132 on blocks of 16)
+    if (p.cache_dtype == HIPATTN_I8 && p.head_dim < kD) return resident;
     if (eight_bit(p.cache_dtype)) return p.head_dim <= 64 ? resident : resident / 4 * 3;
     return resident / 2;
 }

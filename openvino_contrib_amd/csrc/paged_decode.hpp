@@ -312,9 +312,13 @@ __device__ __forceinline__ void load_block_padded(BlockRegs<kU8>& b, const uint8
 
 // A unit of an i8 cache: rows of head_dim codes and nothing between them.  The blocks' scales travel as wavefront-uniform
 // values beside it (UnitScales).
+// At head size 64 a lane holds four columns of V instead of eight (and sixteen lanes then hold the row): eight would leave half of
+// the lanes without any, and the products with as many rows of nothing.
+template <int kHD>
 struct BlockRegsI8 {
+    static constexpr int kValueWords = kHD == 64 ? 1 : 2;
     uint2_t k[2][4];  // as BlockRegs<true>
-    uint2_t v[8];
+    uint32_t v[8][kValueWords];
 };
 // What a tile's block contributes to its scores and probabilities: the key scale times softmax scale and log2(e), log2 of the
 // value scale, and its reciprocal.
@@ -324,7 +328,7 @@ struct UnitScales {
 
 // row: bytes from row to row (kHD unless the head is narrower); koff, voff, v_ok as in load_block_padded.
 template <int kHD, int kBlk, bool kPad>
-__device__ __forceinline__ void load_block_i8(BlockRegsI8& b, const uint8_t* const (&kb)[2], const uint8_t* const (&vb)[2], int row,
+__device__ __forceinline__ void load_block_i8(BlockRegsI8<kHD>& b, const uint8_t* const (&kb)[2], const uint8_t* const (&vb)[2], int row,
                                               const int (&koff)[kHD / 32], int voff, bool v_ok, int n16, int kg) {
 #pragma unroll
     for (int t = 0; t < 2; t++) {
@@ -342,16 +346,16 @@ __device__ __forceinline__ void load_block_i8(BlockRegsI8& b, const uint8_t* con
             }
         }
     }
-    const bool mine = kPad ? v_ok : (kHD == 128 || n16 * 8 < kHD);
-    const int first = kPad ? voff : kg * 4 * kHD + n16 * 8, step = kPad ? row : kHD;
+    constexpr int kWords = BlockRegsI8<kHD>::kValueWords;
+    const int first = kPad ? voff : kg * 4 * kHD + n16 * 4 * kWords, step = kPad ? row : kHD;
 #pragma unroll
     for (int t = 0; t < 2; t++) {
         const uint8_t* const vt = (kBlk == 32 ? vb[0] + t * 16 * step : vb[t]) + first;
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            uint2_t piece = {0u, 0u};
-            if (mine) piece = *(const uint2_t*)(vt + r * step);
-            b.v[t * 4 + r] = piece;
+#pragma unroll
+            for (int w = 0; w < kWords; w++) b.v[t * 4 + r][w] = 0u;
+            if (!kPad || v_ok) __builtin_memcpy(b.v[t * 4 + r], vt + r * step, 4 * kWords);
         }
     }
 }
@@ -359,8 +363,8 @@ __device__ __forceinline__ void load_block_i8(BlockRegsI8& b, const uint8_t* con
 struct WaveState {
     float m;          // running max of the scaled scores (log2 domain), per head (lane & 15)
     float l;          // this lane's share of the running sum
-    float corr;       // u8 only: this lane's share of sum_j p'_j zp_j
-    float4_t acc[8];  // acc[e][r] = O[head][(kg*4 + r)*8 + e]
+    float corr;       // u8 only: this lane's share of sum_j p'_j zp_j (i8: all of sum_j p'_j)
+    float4_t acc[8];  // acc[e][r] = O[head][(kg*4 + r)*8 + e]; i8 at head size 64: e < 4, O[head][(kg*4 + r)*4 + e]
 };
 
 // kTileMask (blocks of 16): `tiles_in` has bit t set when tile t of the unit lies in a block of the
@@ -526,10 +530,16 @@ __device__ __forceinline__ void process_block(WaveState& st, BlockRegs<kU8>& b, 
 // The value scale joins the exponent: the running maximum then bounds what is multiplied with the codes, in fp16 whatever the
 // scales' size, and the row sum takes the probabilities back by 1 / v_scale.  (A u8 row's scale and zero-point cost the u8 form
 // two broadcasts and two more operations for every probability.)
+// sum(p), of the probabilities as they are rounded for the product, is one more product, with ones.  (The row sum takes the unrounded
+// ones: next to a block of large values, those of a block of small ones may round to nothing and still count as weight.)
+// A unit costs 130 vector instructions at head size 64 and 195 at 128; with a comparison for every score, sums of the rounded
+// probabilities lane by lane and eight columns of V to a lane at head size 64 it was 304 and 330.  64 sequences of 512 to 8,192 tokens,
+// 32 heads on 8, blocks of 32, the whole call: head size 64 68.2 us (79.7 before; their bytes take 47.8 at 5.9 TB/s), 128 117.3 (119.4;
+// 95.5), 80 (padded) 89.1 (112; 59.7).
 constexpr float kCodeBias = kByteBias + 128.0f;
 template <int kHD, bool kTileMask>
-__device__ __forceinline__ void process_block_i8(WaveState& st, BlockRegsI8& b, const half8_t (&qf)[4], float sumq, const UnitScales& u, int tok_base,
-                                                 int j0, int ctx, int kg, int tiles_in) {
+__device__ __forceinline__ void process_block_i8(WaveState& st, const BlockRegsI8<kHD>& b, const half8_t (&qf)[4], float sumq, const UnitScales& u,
+                                                 int tok_base, int j0, int ctx, int kg, int tiles_in) {
     const int tiles = kTileMask ? tiles_in : 3;
     using Op = Op16<false>;
     float4_t s[2];
@@ -547,55 +557,53 @@ __device__ __forceinline__ void process_block_i8(WaveState& st, BlockRegsI8& b, 
             s[t] = Op::mma(Op::from_bits(w), qf[i], s[t]);
         }
     }
-    const bool partial = (tok_base < j0) || (tok_base + kUnit > ctx) || tiles != 3;  // wavefront-uniform
     float sv[8];
-    float mloc = -INFINITY;
 #pragma unroll
     for (int t = 0; t < 2; t++) {
         const float off = fmaf(-kCodeBias * sumq, u.key[t], u.value_log2[t]);
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            float x = fmaf(s[t][r], u.key[t], off);
-            if (partial) {
-                const int tok = tok_base + t * 16 + kg * 4 + r;
-                x = (tok >= j0 && tok < ctx && ((tiles >> t) & 1)) ? x : -INFINITY;
-            }
-            sv[t * 4 + r] = x;
-            mloc = fmaxf(mloc, x);
-        }
+        for (int r = 0; r < 4; r++) sv[t * 4 + r] = fmaf(s[t][r], u.key[t], off);
     }
+    if (tok_base < j0 || tok_base + kUnit > ctx || tiles != 3) {  // (scalars: a branch that most units pass by)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int t = e >> 2, tok = tok_base + t * 16 + kg * 4 + (e & 3);
+            sv[e] = (tok >= j0 && tok < ctx && ((tiles >> t) & 1)) ? sv[e] : -INFINITY;
+        }
+        asm volatile("" : "+v"(sv[0]));  // (or all of it is computed for every unit, and selected from)
+    }
+    float mloc = sv[0];
+#pragma unroll
+    for (int e = 1; e < 8; e++) mloc = fmaxf(mloc, sv[e]);
     mloc = max_over_rows(mloc);
     const float m_new = fmaxf(st.m, mloc);  // finite: every processed block holds an attended token
     const float alpha = fast_exp2(st.m - m_new);
     st.m = m_new;
     half8_t pf;
-    float csum = 0.0f, lsum[2] = {0.0f, 0.0f};
+    float lsum[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         const float pj = fast_exp2(sv[j] - m_new);
         lsum[j >> 2] += pj;
         Op::set(pf, j, pj);
-        csum += Op::get(pf, j);
     }
-    st.l = st.l * alpha + fmaf(lsum[0], u.value_inverse[0], lsum[1] * u.value_inverse[1]);
-    st.corr = st.corr * alpha + csum;
+    constexpr int kOut = 4 * BlockRegsI8<kHD>::kValueWords;
     if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) st.acc[e] *= alpha;
+        for (int e = 0; e < kOut; e++) st.acc[e] *= alpha;
     }
+    const half8_t ones = as_half8((uint4_t){0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u});
+    const float4_t sums = Op::mma(ones, pf, (float4_t){0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        b.v[j][0] ^= 0x80808080u;
-        b.v[j][1] ^= 0x80808080u;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
+    for (int e = 0; e < kOut; e++) {
         uint4_t w;
         const uint32_t sel = 0x0c000c00u | ((4u + (e & 3)) << 16) | (uint32_t)(e & 3);
 #pragma unroll
-        for (int jp = 0; jp < 4; jp++) w[jp] = bytes_to_biased_half2(b.v[2 * jp][e >> 2], b.v[2 * jp + 1][e >> 2], sel);
+        for (int jp = 0; jp < 4; jp++) w[jp] = __builtin_amdgcn_perm(b.v[2 * jp + 1][e >> 2], b.v[2 * jp][e >> 2], sel) ^ 0x64806480u;
         st.acc[e] = Op::mma(Op::from_bits(w), pf, st.acc[e]);
     }
+    st.l = st.l * alpha + fmaf(lsum[0], u.value_inverse[0], lsum[1] * u.value_inverse[1]);
+    st.corr = st.corr * alpha + sums[0];
 }
 
 // Length of one (sequence, kv head) segment on the work line: its blocks plus `switch_cost`
@@ -719,7 +727,8 @@ struct MergeArgs {
     int out_dtype, num_heads_q, num_heads_kv, head_dim;
     const float* sinks;
 };
-template <int kHD, bool kPad>
+// kRows: runs of eight columns that a lane holds (4; 2: see BlockRegsI8)
+template <int kHD, bool kPad, int kRows = 4>
 __device__ __forceinline__ void merge_in_kernel(const MergeArgs& p, const Line& line, int s, int h, int token,
                                                 int id_first, int id_last, int lane) {
     const int Hkv = p.num_heads_kv, G = p.num_heads_q / p.num_heads_kv;
@@ -761,7 +770,7 @@ __device__ __forceinline__ void merge_in_kernel(const MergeArgs& p, const Line& 
                 const int64_t slot = (int64_t)id + (int64_t)s * Hkv + h;
                 const float* rec = p.part_out + (slot * kPartPairs * 4 * G + (kg * G + n16)) * 2;
 #pragma unroll
-                for (int r = 0; r < 4; r++)
+                for (int r = 0; r < kRows; r++)
 #pragma unroll
                     for (int e2 = 0; e2 < 4; e2++) {
                         float x, y;
@@ -787,9 +796,9 @@ __device__ __forceinline__ void merge_in_kernel(const MergeArgs& p, const Line& 
     if (p.sinks != nullptr && l_run > 0.0f) l_run += fast_exp2(p.sinks[h * G + n16] * kLog2e - m_run);
     const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-        const int d0 = (kg * 4 + r) * 8;
-        if ((kPad || kHD < 128) && d0 >= head_dim) continue;
+    for (int r = 0; r < kRows; r++) {
+        const int d0 = (kg * kRows + r) * 8;
+        if ((kPad || kRows * 32 > kHD) && d0 >= head_dim) continue;
         float o[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) o[e] = acc[e][r] * inv;
@@ -821,6 +830,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams& p, const Kv
     static_assert(!kAlibi || (kWaves == 1 && !kSelfPlan), "the distance bias (p.alibi_slopes) exists in the ordinary launch only");
     // kI8: a cache of codes with a scale per block and kv head; it shares what holds for both 8-bit caches (kU8)
     static_assert(!kI8 || (kU8 && !kAlibi), "i8 caches: an 8-bit form, without the distance bias");
+    constexpr int kRows = kI8 && kHD == 64 ? 2 : 4;  // runs of eight columns of the result that a lane holds (BlockRegsI8)
     // The merge inside the kernel (p.fused_merge) is built into the u8 instantiations only: the 16-bit ones use
     // every register in their loop, and with that code behind the loop the allocator spilled 29 of them.
     constexpr bool kFusedBuilt = kU8;
@@ -903,8 +913,8 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams& p, const Kv
             const int first = kg * (kHD / 4) + i * 8;  // first of the piece's eight columns
             koff[i] = n16 * (int)kRowBytes + (kU8 ? kRowHead + (first < head_dim ? first : 0) : (first < head_dim ? first * 2 : 0));
         }
-        voff = kg * 4 * (int)kRowBytes + (kU8 ? kRowHead + n16 * 8 : n16 * 16);
-        v_ok = n16 * 8 < head_dim;
+        voff = kg * 4 * (int)kRowBytes + (kU8 ? kRowHead + n16 * 2 * kRows : n16 * 16);
+        v_ok = n16 * 2 * kRows < head_dim;
     }
 
     // The static piece first, then dynamic pieces for as long as there are any.  The ticket for
@@ -942,11 +952,17 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams& p, const Kv
             rg = plan_rec[s];
         else
             rg = ((const DecodeRange*)p.seq_info)[s];
+        // (i8: what the lanes share kept where it takes no vector instruction)
+        const auto shared = [](int x) __attribute__((always_inline)) { return kI8 ? __builtin_amdgcn_readfirstlane(x) : x; };
+        if constexpr (kI8) {
+            rg.j0 = shared(rg.j0);
+            rg.ctx = shared(rg.ctx);
+        }
         const int nb = rg.nb;
         if (nb <= 0) break;  // cannot happen for a consistent plan; never loop forever
         const int seglen = nb + p.switch_cost;
         const int64_t seq_L0 = (int64_t)prefix_at(s) * Hkv;
-        const int h = (int)((L - seq_L0) / seglen);
+        const int h = shared((int)((L - seq_L0) / seglen));
         const int64_t seg_B0 = seq_L0 + (int64_t)h * seglen + p.switch_cost;  // line position of the segment's block 0
         const int64_t seg_L1 = seg_B0 + nb;                        // end of the segment
         const int64_t from = max(L, seg_B0), to = min(L_end, seg_L1);
@@ -954,8 +970,8 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams& p, const Kv
             L = to;
             continue;
         }
-        const int b_rel = (int)(from - seg_B0);
-        const int n = (int)(to - from);  // blocks of this segment in this piece
+        const int b_rel = shared((int)(from - seg_B0));
+        const int n = shared((int)(to - from));  // blocks of this segment in this piece
         const bool whole = (n == nb);
         L = from;
         // the segment ends here and began in an earlier piece: this piece combines it when it is done
@@ -1051,7 +1067,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams& p, const Kv
                 }
                 return u;
             };
-            using Regs = typename std::conditional<kI8, BlockRegsI8, BlockRegs<kU8>>::type;
+            using Regs = typename std::conditional<kI8, BlockRegsI8<kHD>, BlockRegs<kU8>>::type;
             // which tiles of unit i were issued (0: none, the unit is skipped); never reads outside the cache
             auto issue = [&](Regs& regs, int i) -> int {
                 if constexpr (kEntries == 1) {
@@ -1137,28 +1153,29 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams& p, const Kv
         float l = st.l, corr = st.corr;
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
-        if constexpr (kU8) {
+        if constexpr (kI8) {
+            corr *= kCodeBias;
+        } else if constexpr (kU8) {
             corr += __shfl_xor(corr, 16, 64);
             corr += __shfl_xor(corr, 32, 64);
-            if constexpr (kI8) corr *= kCodeBias;
         }
         const int64_t slot = (int64_t)piece + (int64_t)s * Hkv + h;  // unique per (piece, segment)
         if (n16 < G) {
             if (whole && p.sinks != nullptr && l > 0.0f) l += fast_exp2(p.sinks[h * G + n16] * kLog2e - st.m);
             const float inv = whole ? (l > 0.0f ? 1.0f / l : 0.0f) : 1.0f;
-            // acc[e][r] is head-dim (kg*4 + r)*8 + e: eight consecutive outputs per r
+            // acc[e][r] is head-dim (kg*4 + r)*8 + e: eight consecutive outputs per r (kRows == 2: (kg*4 + r)*4 + e, eight per two r)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
+            for (int r = 0; r < kRows; r++) {
                 float o[8];
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    float v = st.acc[e][r];
+                    float v = kRows == 4 ? st.acc[e][r] : st.acc[e & 3][2 * r + (e >> 2)];
                     if constexpr (kU8) v -= corr;
                     o[e] = v * inv;
                 }
-                const int d0 = (kg * 4 + r) * 8;
+                const int d0 = (kg * kRows + r) * 8;
                 // (rows of the accumulator beyond the head size hold nothing; a fused partial carries them all the same)
-                if ((kPad || kHD < 128) && d0 >= head_dim && (whole || !(kFusedBuilt && p.fused_merge))) continue;
+                if ((kPad || kRows * 32 > kHD) && d0 >= head_dim && (whole || !(kFusedBuilt && p.fused_merge))) continue;
                 if (whole) {
                     store_out8(p.out, ((int64_t)rg.token * p.num_heads_q + h * G + n16) * head_dim + d0, p.out_dtype, o);
                 } else if (kFusedBuilt && p.fused_merge) {
@@ -1197,7 +1214,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams& p, const Kv
             mr = ((const DecodeRange*)p.seq_info)[ms];
         const int64_t first_unit = (int64_t)prefix_at(ms) * Hkv + (int64_t)mh * (mr.nb + p.switch_cost) + p.switch_cost;
         const MergeArgs ma = {p.part_out, p.part_ml, p.part_flag, p.merge_tag, p.out, p.out_dtype, p.num_heads_q, p.num_heads_kv, p.head_dim, p.sinks};
-        merge_in_kernel<kHD, kPad>(ma, line, ms, mh, mr.token, line.piece_at(first_unit), piece, lane);
+        merge_in_kernel<kHD, kPad, kRows>(ma, line, ms, mh, mr.token, line.piece_at(first_unit), piece, lane);
         merge_seg = -1;
     }
     if (p.dyn_pieces <= 0) break;
