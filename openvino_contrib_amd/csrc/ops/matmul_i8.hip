@@ -91,32 +91,34 @@ hipattn_status checked(const hipops_matmul_i8_desc* d) {
 
 int64_t bytes_of_parts(int64_t m, int64_t n, int parts) { return parts > 1 ? parts * m * ((n + 3) / 4 * 4) * 4 : 0; }
 
-// Which kernel, and how many parts of k: the least time by a model of what was measured (us; bf16 results, three sets of operands in
-// turn), over 160 sizes: m of 1 to 8,192 on weights of 4,096 x 4,096, 28,672 x 4,096, 11,008 x 4,096, 4,096 x 14,336, 2,560 x 10,240, 1,024 x
-// 4,096, 6,144 x 4,096 and 2,048, 512 x 2,048, 320 and 2,048 x 1,024, 128 x 8,192.  Its choice is 0.9 % from the best of all choices on
-// average, 22 % at worst (128 rows of 512 x 2,048: 9.5 for 7.8).
+// Which kernel, and how many parts of k: the least time by a model of what was measured (us; bf16 results, the weights of each call
+// others than those of the calls before, 768 MB of them in turn, the activations the same), over 291 sizes: m of 1 to 8,192 on weights of 4,096 x
+// 4,096, 28,672 x 4,096, 11,008 x 4,096, 4,096 x 14,336, 5,120 x 13,824, 2,560 x 10,240, 1,024 x 4,096, 6,144 x 4,096 and 2,048, 512 x 2,048, 320
+// and 2,048 x 1,024, 128 x 8,192.  Its choice is 0.5 % from the best of all choices on average, 15 % at worst (256 x 4,096 x 4,096: 20.3 for 17.7).
+// (Fitted to calls whose weights had stayed in the last cache, it was 2.3 % off on average and 64 % at worst.)
 // A tile costs its start and end, and for each stage of 128 bytes of k the largest of: what a compute unit takes that has one tile
 // (`alone`: the loads it waits for); with more tiles than compute units, what the fullest takes (`together`) and the whole device
 // (`through`: power and the caches).  The operands' bytes bound it from below.  Parts of k cost the second launch and their sums' way
-// through memory.  Where the sides cross (us): 64 x 4,096 x 4,096 tiles of 32 rows in four parts 12.4, of 64 in four 13.1, of 128 14.0;
-// 512 x 4,096 x 4,096 tiles of 64 18.7, of 128 with a deep ring 21.2, of 128 26.8, of 256 33; 1,024 x 6,144 x 4,096 of 128 35.6, deep 43.0, of
-// 256 52.7; 1,111 x 4,096 x 14,336 of 128 90, of 256 in three parts 91; 3,000 x 4,096 x 14,336 of 256 190, of 128 209; 8,192 x 6,144 x 4,096
-// of 256 205, of 128 236; 16 x 4,096 x 4,096 without LDS 7.9, with 10.3; 16 x 28,672 x 4,096 38.0 and 26.9.
+// through memory.  Where the sides cross (us, m x n x k): 64 x 4,096 x 4,096 tiles of 32 rows in four parts 13.5, of 64 in six 13.8; 512 x 4,096
+// x 4,096 of 64 20.6, of 128 with a deep ring 22.8, of 128 in four parts 28.6, of 256 in six 34.4; 600 x 5,120 x 13,824 of 128 with a deep ring
+// 61.3, of 256 in four parts 69.1, of 128 in two 70.8, of 64 84.9; 1,024 x 6,144 x 4,096 of 128 42.3, deep 45.4, of 256 in two parts 54.6; 1,111 x
+// 4,096 x 14,336 of 256 in three parts 93.9, of 128 109; 1,500 x 4,096 x 14,336 of 128 112, of 256 in two parts 117; 3,000 x 4,096 x 14,336 of 256
+// 174, of 128 201; 8,192 x 6,144 x 4,096 of 256 198, of 128 243; 16 x 4,096 x 4,096 without LDS 8.0, with 10.9; 16 x 28,672 x 4,096 38.3 and 24.9.
 struct TileCost {
     I8Tile tile;
     int rows, columns, most_rows;  // tiles of more rows than this are never the faster ones
     float start, alone, together, through;
 };
 constexpr TileCost kTileCosts[] = {
-    {kI8Tile32, 32, 128, 128, 3.7f, 0.41f, 0.32f, 0.28f},           {kI8Tile64, 64, 128, 1600, 4.1f, 0.43f, 0.29f, 0.46f},
-    {kI8Tile128Deep, 128, 128, 1 << 30, 5.1f, 0.52f, 0.66f, 0.60f}, {kI8Tile128, 128, 128, 1 << 30, 7.0f, 0.67f, 0.37f, 0.59f},
-    {kI8Tile256, 256, 256, 1 << 30, 11.7f, 1.39f, 1.53f, 1.91f},
+    {kI8Tile32, 32, 128, 128, 3.94f, 0.434f, 0.534f, 0.517f},           {kI8Tile64, 64, 128, 1600, 4.48f, 0.449f, 0.388f, 0.483f},
+    {kI8Tile128Deep, 128, 128, 1 << 30, 5.15f, 0.527f, 0.648f, 0.560f}, {kI8Tile128, 128, 128, 1 << 30, 6.42f, 0.775f, 0.505f, 0.534f},
+    {kI8Tile256, 256, 256, 1 << 30, 12.5f, 1.14f, 1.66f, 1.37f},
 };
 // Rows at any address, through registers (us, tiles of 32 rows / 128 rows at their best parts: 64 x 4,095 x 4,095 16.8 / -; 512 x 4,095 x 4,095
 // 39.6 / 37.1; 128 x 4,095 x 14,333 38.9 / 34.9; 100 x 2,001 x 1,001 10.4 / 17.8; 8,191 x 6,143 x 4,097 - / 391).
 constexpr TileCost kAnyCosts[] = {{kI8Any32, 32, 128, 512, 3.8f, 0.90f, 0.55f, 0.55f}, {kI8Any128, 128, 128, 1 << 30, 6.5f, 1.65f, 0.94f, 0.94f}};
 constexpr int kParts[] = {1, 2, 3, 4, 6, 8, 12, 16};
-constexpr float kUnits = 256.0f, kBytesPerUs = 5.95e6f, kSumBytesPerUs = 3.8e6f, kSecondLaunch = 2.7f;
+constexpr float kUnits = 256.0f, kBytesPerUs = 8.0e6f, kSumBytesPerUs = 3.88e6f, kSecondLaunch = 2.88f;
 
 I8Plan plan_of(int64_t m, int64_t n, int64_t k, size_t workspace_bytes, bool aligned) {
     I8Plan best{aligned ? kI8Tile32 : kI8Any32, 1};
@@ -140,7 +142,7 @@ I8Plan plan_of(int64_t m, int64_t n, int64_t k, size_t workspace_bytes, bool ali
     }
     if (m <= 16) {
         const float steps = (float)k / 2048.0f, rounds = ceilf((float)n / 16.0f / kUnits);
-        least = 3.9f + std::max({0.41f * steps, 0.365f * rounds * steps * (1.0f + (float)m / 32.0f), (float)n * (float)k / 4.7e6f});
+        least = 3.98f + std::max({0.275f * steps, 0.565f * rounds * steps * (1.0f + 0.134f * (float)m), (float)n * (float)k / 5.76e6f});
         best = {kI8Few, 1};
     }
     for (const TileCost& t : kTileCosts) consider(t);
