@@ -135,8 +135,6 @@ struct PagedParams {
     const void* q;
     const uint8_t* key_cache;
     const uint8_t* value_cache;
-    const float* key_scales;    // HIPATTN_I8: [num_blocks, the cache's kv heads]
-    const float* value_scales;
     const int32_t* past_lens;
     const int32_t* subsequence_begins;
     const int32_t* block_indices;
@@ -200,12 +198,15 @@ struct PagedParams {
     uint16_t* shadow_k;
     uint16_t* shadow_v;
     int32_t* shadow_table;
+    int tiles_only;       // (flash_small.hip) tile_prefix counts single-token sequences too: there are no decode rows
+    int lone_tile;        // (paged_mixed.hip) one sequence, which gets query tiles also if it is a single token: no decode rows, no merge
+    // (the i8 caches' fields stand last, where the other caches' kernels find their arguments as they were without them)
+    const float* key_scales;    // HIPATTN_I8: [num_blocks, the cache's kv heads]
+    const float* value_scales;
     // i8 caches: sequences of kShadowTokens new tokens or more, cached tokens included; a sequence's blocks from shadow_base[s] on (-1: none),
     // beginning with the first that its window leaves; shadow_capacity blocks in all
     int32_t* shadow_base;
     int shadow_capacity;
-    int tiles_only;       // (flash_small.hip) tile_prefix counts single-token sequences too: there are no decode rows
-    int lone_tile;        // (paged_mixed.hip) one sequence, which gets query tiles also if it is a single token: no decode rows, no merge
 };
 
 // A shorter prompt is read by few query tiles and costs the writer as much (32 heads on 8, us without -> with: 8 prompts of 100 21.2 -> 23.0, of 300
