@@ -11,7 +11,8 @@ namespace {
 
 // Up to 16 activation rows: the weights, read once, are all of the time.  A workgroup takes 16 weight rows and its eight wavefronts an
 // eighth of k each; a lane's loads are the matrix operands as they stand (16 bytes of k of weight row lane % 16, activations
-// alike), kGroup steps multiplied while the next ones are on their way.  Only the eight partial sums meet in LDS.
+// alike), kFewGroup steps multiplied while the next ones are on their way.  Only the eight partial sums meet in LDS.  One row on
+// 4,096 x 4,096 6.0 us (2.8 TB/s: launch and one round of loads; in tiles 10.9), on 4,096 x 14,336 14.3.
 constexpr int kFewWaves = 8, kFewGroup = 4;
 
 __global__ __launch_bounds__(64 * kFewWaves) void matmul_i8_few_kernel(MatmulI8Params p) {

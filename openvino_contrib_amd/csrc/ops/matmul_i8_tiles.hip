@@ -1,4 +1,16 @@
-// Products of 8-bit codes in tiles through LDS (hipops_matmul_i8, rows at multiples of 16 bytes).
+// Products of 8-bit codes in tiles through LDS (hipops_matmul_i8).
+//
+//   c[i, j] = a_scale[i] b_scale[j] sum_l a[i, l] b[j, l] + bias[j] + residual[i, j]
+// Sums on v_mfma_i32_32x32x32_i8, exact; the rest in fp32, rounded once, on the accumulators.
+//
+// With few activation rows the weights' bytes bound it, with many the matrix cores.  Tiles of 32, 64, 128 and 256 activation rows on 128 (256) weight
+// rows: a large one reads less from L2 and LDS for a product, small ones fill the device; k in parts where even those do not, whose sums a second
+// launch adds (matmul_i8.hip has the rule and where the sides cross).  A stage is 128 bytes of k, loaded straight to LDS while the one or two
+// before it are multiplied (rows at any address: through registers).  8,192 x 8,192 x 8,192 502 us (2.19 POP/s; a library's product of the same 535),
+// 8,192 x 6,144 x 4,096 205 (190), 64 x 28,672 x 4,096 27 (4.4 TB/s of weights), 1,111 x 4,096 x 14,336 94 in three parts.  At the large sizes the matrix
+// cores are busy 48 % of the time at 1.95 GHz (2.4 without load): loads alone take 169 of the 205 us, products alone 175, 135 on operands of
+// zeros.  Slower there: stages of 64 bytes, five on their way (220), four wavefronts of 128 x 128 (342), rows touched in the L2 a stage
+// ahead (212 to 216).  Parts added by the workgroup that is last to be done with its own, without a second launch: 5.5 % slower over 291 sizes.
 #include "ops/matmul_i8.hpp"
 
 namespace hipops {
