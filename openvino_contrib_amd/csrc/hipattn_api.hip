@@ -526,6 +526,11 @@ HIPATTN_EXPORT hipattn_status hipattn_rope_append(const hipattn_pa_desc* desc, c
     const bool by_token = out_token >= (desc->num_heads_q - 1) * out_head + desc->head_dim && out_head >= desc->head_dim;
     const bool by_head = out_head >= (int64_t)(desc->num_tokens - 1) * out_token + desc->head_dim && out_token >= desc->head_dim;
     if (q_out && !by_token && !by_head) return fail(HIPATTN_INVALID_ARGUMENT, "rope_append: rows of q_out overlap");
+    // (in place: a row that lay elsewhere afterwards could be another's that is still to be read)
+    const int64_t q_head = r.q_head_stride ? r.q_head_stride : desc->head_dim, q_token = r.q_token_stride ? r.q_token_stride : (int64_t)desc->num_heads_q * desc->head_dim;
+    if (q && q == q_out && (q_head != out_head || q_token != out_token))
+        return fail(HIPATTN_INVALID_ARGUMENT, "rope_append: in place with rows %lld, %lld apart and %lld, %lld afterwards", (long long)q_token, (long long)q_head,
+                    (long long)out_token, (long long)out_head);
     if (desc->num_tokens == 0 || desc->num_seqs == 0) return HIPATTN_OK;
     if (!k_new || !v_new || !key_cache || !value_cache || !past_lens || !subsequence_begins || !block_indices || !block_indices_begins)
         return fail(HIPATTN_INVALID_ARGUMENT, "rope_append: null pointer");

@@ -1,5 +1,5 @@
 // Products of 8-bit codes (hipops_matmul_i8): c = a_scale b_scale (A B^T) + bias + residual, sums exact in 32-bit integers on the
-// matrix cores.  The entry, the choice among the kernels, and the one for up to 16 activation rows; the others: matmul_i8_tiles.hip.
+// matrix cores.  The entry, the choice among the kernels, and the one for up to 32 activation rows; the others: matmul_i8_tiles.hip.
 #include <algorithm>
 #include <cmath>
 
@@ -9,71 +9,112 @@ namespace hipops {
 
 namespace {
 
-// Up to 16 activation rows: the weights, read once, are all of the time.  A workgroup takes 16 weight rows and its eight wavefronts an
-// eighth of k each; a lane's loads are the matrix operands as they stand (16 bytes of k of weight row lane % 16, activations
-// alike), kFewGroup steps multiplied while the next ones are on their way.  Only the eight partial sums meet in LDS.  One row on
-// 4,096 x 4,096 6.0 us (2.8 TB/s: launch and one round of loads; in tiles 10.9), on 4,096 x 14,336 14.3.
-constexpr int kFewWaves = 8, kFewGroup = 4;
+// Up to 32 activation rows: the weights, read once, are most of the time.  A workgroup takes 16 kN weight rows and its eight wavefronts an
+// eighth of k each; a lane's loads are the matrix operands as they stand (16 bytes of k of weight row lane % 16, of kM tiles of 16 activation
+// rows alike), kGroup steps multiplied while the next ones are on their way.  Only the eight partial sums meet in LDS.  One row on
+// 4,096 x 4,096 6.0 us alone (2.8 TB/s: launch and one round of loads; in tiles with LDS 10.1), 32 rows 10.1 (11.5), 64 14.2 (13.4): every workgroup
+// reads all activations, 16 bytes of 16 rows at a time.  Twice the weight rows halve that, where n still fills the device: 32 x 6,144 x 2,048
+// 10.1 -> 8.6 us (in tiles 10.7), 16 x 28,672 x 4,096 38.4 -> 33.0 (25.0).
+constexpr int kFewWaves = 8;
 
+template <int kM, int kN>
 __global__ __launch_bounds__(64 * kFewWaves) void matmul_i8_few_kernel(MatmulI8Params p) {
-    __shared__ int4_t sums[kFewWaves][64];
+    constexpr int kGroup = 4;
+    static_assert(kM * kN <= kFewWaves, "a wavefront for each tile of the result");
+    __shared__ int4_t sums[kFewWaves][kM * kN][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, row = lane & 15, quarter = lane >> 4;
-    const int64_t n0 = 16 * (int64_t)blockIdx.x;
+    const int64_t n0 = 16 * kN * (int64_t)blockIdx.x;
     const int steps = (int)((p.k + 63) / 64);
     const int first = steps * wave / kFewWaves, last = steps * (wave + 1) / kFewWaves;
-    const int8_t* const w = p.b + min(n0 + row, p.n - 1) * p.ldb + 16 * quarter;
-    const int8_t* const x = p.a + (int64_t)min((int64_t)row, p.m - 1) * p.lda + 16 * quarter;
-    const bool real = row < p.m;
+    const int8_t *w[kN], *x[kM];
+#pragma unroll
+    for (int j = 0; j < kN; j++) w[j] = p.b + min(n0 + 16 * j + row, p.n - 1) * p.ldb + 16 * quarter;
+#pragma unroll
+    for (int i = 0; i < kM; i++) x[i] = p.a + min((int64_t)(16 * i + row), p.m - 1) * p.lda + 16 * quarter;
+    const bool real = kM > 1 || row < p.m;  // (a single tile: lanes without a row load nothing)
     const int whole = (int)((p.k - 16 * quarter + 48) / 64);  // steps in which this lane has a piece (k is a multiple of 16)
-    int4_t acc = {0, 0, 0, 0};
+    int4_t acc[kN][kM];
+#pragma unroll
+    for (int j = 0; j < kN; j++)
+#pragma unroll
+        for (int i = 0; i < kM; i++) acc[j][i] = (int4_t){0, 0, 0, 0};
     struct Group {
-        uint4_t w[kFewGroup], x[kFewGroup];
+        uint4_t w[kGroup][kN], x[kGroup][kM];
     } now, next;
     const auto load = [&](Group& g, int s) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < kFewGroup; u++) {
+        for (int u = 0; u < kGroup; u++) {
             const int at = min(s + u, last - 1);  // (past the end: unused)
-            g.w[u] = (uint4_t){0u, 0u, 0u, 0u};
-            if (at < whole) g.w[u] = *(const uint4_t*)(w + 64 * (int64_t)at);
+#pragma unroll
+            for (int j = 0; j < kN; j++) {
+                g.w[u][j] = (uint4_t){0u, 0u, 0u, 0u};
+                if (at < whole) g.w[u][j] = *(const uint4_t*)(w[j] + 64 * (int64_t)at);
+            }
         }
         if (real) {
 #pragma unroll
-            for (int u = 0; u < kFewGroup; u++) {
+            for (int u = 0; u < kGroup; u++) {
                 const int at = min(s + u, last - 1);
-                if (at < whole) g.x[u] = *(const uint4_t*)(x + 64 * (int64_t)at);
+#pragma unroll
+                for (int i = 0; i < kM; i++)
+                    if (at < whole) g.x[u][i] = *(const uint4_t*)(x[i] + 64 * (int64_t)at);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
     };
     const auto multiply = [&](const Group& g, int s) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < kFewGroup; u++)
-            if (s + u < last) acc = mma_i8_16(g.w[u], g.x[u], acc);
+        for (int u = 0; u < kGroup; u++)
+            if (s + u < last) {
+#pragma unroll
+                for (int j = 0; j < kN; j++)
+#pragma unroll
+                    for (int i = 0; i < kM; i++) acc[j][i] = mma_i8_16(g.w[u][j], g.x[u][i], acc[j][i]);
+            }
         __builtin_amdgcn_sched_barrier(0);
     };
 #pragma unroll
-    for (int u = 0; u < kFewGroup; u++) now.x[u] = next.x[u] = (uint4_t){0u, 0u, 0u, 0u};  // (lanes without a row keep these)
+    for (int u = 0; u < kGroup; u++)
+#pragma unroll
+        for (int i = 0; i < kM; i++) now.x[u][i] = next.x[u][i] = (uint4_t){0u, 0u, 0u, 0u};  // (lanes without a row or a piece keep these)
     if (first < last) {
         load(now, first);
-        for (int s = first; s < last; s += 2 * kFewGroup) {
-            if (s + kFewGroup < last) load(next, s + kFewGroup);
+        for (int s = first; s < last; s += 2 * kGroup) {
+            if (s + kGroup < last) load(next, s + kGroup);
             multiply(now, s);
-            if (s + 2 * kFewGroup < last) load(now, s + 2 * kFewGroup);
-            multiply(next, s + kFewGroup);
+            if (s + 2 * kGroup < last) load(now, s + 2 * kGroup);
+            multiply(next, s + kGroup);
         }
     }
-    // register r: weight row 4 quarter + r, activation row lane % 16
-    sums[wave][lane] = acc;
-    __syncthreads();
-    if (wave != 0 || !real) return;
-    int4_t sum = sums[0][lane];
+    // register r: weight row 4 quarter + r, activation row lane % 16 of a tile
 #pragma unroll
-    for (int i = 1; i < kFewWaves; i++) sum += sums[i][lane];
+    for (int j = 0; j < kN; j++)
+#pragma unroll
+        for (int i = 0; i < kM; i++) sums[wave][j * kM + i][lane] = acc[j][i];
+    __syncthreads();
+    if (wave >= kM * kN) return;
+    const int64_t to_row = 16 * (wave % kM) + row, to_column = n0 + 16 * (wave / kM) + 4 * quarter;
+    if (to_row >= p.m) return;
+    int4_t sum = sums[0][wave][lane];
+#pragma unroll
+    for (int i = 1; i < kFewWaves; i++) sum += sums[i][wave][lane];
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-        const int64_t column = n0 + 4 * quarter + r;
-        if (column < p.n) store_scalar(p.c, row * p.ldc + column, p.c_dtype, finished(p, sum[r], row, column, p.b_scales ? p.b_scales[column] : 1.0f));
+        const int64_t column = to_column + r;
+        if (column < p.n)
+            store_scalar(p.c, to_row * p.ldc + column, p.c_dtype, finished(p, sum[r], to_row, column, p.b_scales ? p.b_scales[column] : 1.0f));
     }
+}
+
+template <int kM, int kN>
+void launch_few(const MatmulI8Params& p, hipStream_t stream) {
+    hipLaunchKernelGGL((matmul_i8_few_kernel<kM, kN>), dim3((unsigned)((p.n + 16 * kN - 1) / (16 * kN))), dim3(64 * kFewWaves), 0, stream, p);
+}
+void launch_few(const MatmulI8Params& p, bool wide, hipStream_t stream) {
+    if (p.m <= 16)
+        wide ? launch_few<1, 2>(p, stream) : launch_few<1, 1>(p, stream);
+    else
+        wide ? launch_few<2, 2>(p, stream) : launch_few<2, 1>(p, stream);
 }
 
 bool float_dtype(int d) { return d == HIPATTN_F32 || d == HIPATTN_F16 || d == HIPATTN_BF16; }
@@ -93,9 +134,9 @@ hipattn_status checked(const hipops_matmul_i8_desc* d) {
 int64_t bytes_of_parts(int64_t m, int64_t n, int parts) { return parts > 1 ? parts * m * ((n + 3) / 4 * 4) * 4 : 0; }
 
 // Which kernel, and how many parts of k: the least time by a model of what was measured (us; bf16 results, the weights of each call
-// others than those of the calls before, 768 MB of them in turn, the activations the same), over 291 sizes: m of 1 to 8,192 on weights of 4,096 x
+// others than those of the calls before, 768 MB of them in turn, the activations the same), over 330 sizes: m of 1 to 8,192 on weights of 4,096 x
 // 4,096, 28,672 x 4,096, 11,008 x 4,096, 4,096 x 14,336, 5,120 x 13,824, 2,560 x 10,240, 1,024 x 4,096, 6,144 x 4,096 and 2,048, 512 x 2,048, 320
-// and 2,048 x 1,024, 128 x 8,192.  Its choice is 0.5 % from the best of all choices on average, 15 % at worst (256 x 4,096 x 4,096: 20.3 for 17.7).
+// and 2,048 x 1,024, 128 x 8,192.  Its choice is 0.7 % from the best of all choices on average, 15 % at worst (256 x 4,096 x 4,096: 20.3 for 17.7).
 // (Fitted to calls whose weights had stayed in the last cache, it was 2.3 % off on average and 64 % at worst.)
 // A tile costs its start and end, and for each stage of 128 bytes of k the largest of: what a compute unit takes that has one tile
 // (`alone`: the loads it waits for); with more tiles than compute units, what the fullest takes (`together`) and the whole device
@@ -104,7 +145,8 @@ int64_t bytes_of_parts(int64_t m, int64_t n, int parts) { return parts > 1 ? par
 // x 4,096 of 64 20.6, of 128 with a deep ring 22.8, of 128 in four parts 28.6, of 256 in six 34.4; 600 x 5,120 x 13,824 of 128 with a deep ring
 // 61.3, of 256 in four parts 69.1, of 128 in two 70.8, of 64 84.9; 1,024 x 6,144 x 4,096 of 128 42.3, deep 45.4, of 256 in two parts 54.6; 1,111 x
 // 4,096 x 14,336 of 256 in three parts 93.9, of 128 109; 1,500 x 4,096 x 14,336 of 128 112, of 256 in two parts 117; 3,000 x 4,096 x 14,336 of 256
-// 174, of 128 201; 8,192 x 6,144 x 4,096 of 256 198, of 128 243; 16 x 4,096 x 4,096 without LDS 8.0, with 10.9; 16 x 28,672 x 4,096 38.3 and 24.9.
+// 174, of 128 201; 8,192 x 6,144 x 4,096 of 256 198, of 128 243; 24 x 4,096 x 4,096 without LDS 9.2, with 11.0; 24 x 6,144 x 4,096 12.5
+// (wide) and 13.0; 16 x 28,672 x 4,096 33.0 (wide) and 25.0.
 struct TileCost {
     I8Tile tile;
     int rows, columns, most_rows;  // tiles of more rows than this are never the faster ones
@@ -141,10 +183,12 @@ I8Plan plan_of(int64_t m, int64_t n, int64_t k, size_t workspace_bytes, bool ali
         for (const TileCost& t : kAnyCosts) consider(t);
         return best;
     }
-    if (m <= 16) {
-        const float steps = (float)k / 2048.0f, rounds = ceilf((float)n / 16.0f / kUnits);
-        least = 3.98f + std::max({0.275f * steps, 0.565f * rounds * steps * (1.0f + 0.134f * (float)m), (float)n * (float)k / 5.76e6f});
-        best = {kI8Few, 1};
+    if (m <= 32) {
+        const float steps = (float)k / 2048.0f, rows = (float)m, bytes = (float)n * (float)k;
+        const float narrow = 3.88f + std::max({0.808f * steps * (1.0f + 0.0772f * rows), 0.962f * ceilf((float)n / (16.0f * kUnits)) * steps * (1.0f + 0.0527f * rows), bytes / 5.68e6f});
+        const float wide = 3.69f + std::max({2.24f * steps * (1.0f + 0.0311f * rows), 1.29f * ceilf((float)n / (32.0f * kUnits)) * steps * (1.0f + 0.0786f * rows), bytes / 5.37e6f});
+        least = std::min(narrow, wide);
+        best = {wide < narrow ? kI8FewWide : kI8Few, 1};
     }
     for (const TileCost& t : kTileCosts) consider(t);
     return best;
@@ -173,8 +217,8 @@ hipattn_status matmul_i8(const hipops_matmul_i8_desc* d, const int8_t* a, const 
     const bool aligned = (((uintptr_t)a | (uintptr_t)b | (uintptr_t)p.lda | (uintptr_t)p.ldb | (uintptr_t)p.k) & 15) == 0 && p.lda <= (1 << 23) && p.ldb <= (1 << 23);
     const I8Plan plan = plan_of(p.m, p.n, p.k, workspace ? workspace_bytes : 0, aligned);
     hipError_t e = hipSuccess;
-    if (plan.tile == kI8Few) {
-        hipLaunchKernelGGL(matmul_i8_few_kernel, dim3((unsigned)((p.n + 15) / 16)), dim3(64 * kFewWaves), 0, stream, p);
+    if (plan.tile == kI8Few || plan.tile == kI8FewWide) {
+        launch_few(p, plan.tile == kI8FewWide, stream);
         e = hipGetLastError();
     } else {
         e = launch_matmul_i8_tiles(p, plan, workspace, stream);

@@ -36,8 +36,7 @@ __device__ __forceinline__ int4_t mma_i8_16(uint4_t a, uint4_t b, int4_t c) {
 }
 
 __device__ __forceinline__ float finished(const MatmulI8Params& p, int sum, int64_t i, int64_t j, float b_scale) {
-    float x = (float)sum * ((p.a_scales ? p.a_scales[i] : 1.0f) * b_scale);
-    if (p.bias) x += load_scalar(p.bias, j, p.c_dtype);
+    float x = fmaf((float)sum, (p.a_scales ? p.a_scales[i] : 1.0f) * b_scale, p.bias ? load_scalar(p.bias, j, p.c_dtype) : 0.0f);
     if (p.residual) x += load_scalar(p.residual, i * p.ldc + j, p.c_dtype);
     return x;
 }
@@ -84,7 +83,7 @@ __device__ __forceinline__ void store_columns(const MatmulI8Params& p, int64_t t
 }
 
 // ---- how a product is laid out over workgroups ----------------------------------------------------
-enum I8Tile { kI8Any32, kI8Few, kI8Tile32, kI8Tile64, kI8Tile128, kI8Tile256, kI8Tile128Deep, kI8Any128 };
+enum I8Tile { kI8Any32, kI8Few, kI8Tile32, kI8Tile64, kI8Tile128, kI8Tile256, kI8Tile128Deep, kI8Any128, kI8FewWide };  // (the two without LDS: 16 or 32 weight rows to a workgroup)
 struct I8Plan {
     I8Tile tile;
     int parts;  // of k, whose sums meet in the workspace

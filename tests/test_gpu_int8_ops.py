@@ -279,6 +279,15 @@ def test_on_a_stream_of_its_own_and_captured(hip, ops):  # noqa: F811
     stream.close()
 
 
+@pytest.mark.parametrize("m", [1, 15, 16, 17, 24, 31, 32, 33])
+def test_products_of_few_rows(hip, ops, m):  # noqa: F811
+    """Up to 32 rows: one and two tiles of activations, 16 and 32 weight rows to a workgroup (n that fills the device with either), steps that
+    end inside a lane's quarter; the results of calls with and without a workspace are the same to the bit."""
+    for n, k in ((5, 16), (16, 48), (17, 80), (4096, 2048), (6144, 2048), (6145, 64), (8190, 528), (12300, 1040), (128, 8192)):
+        product(hip, ops, m, n, k, BF16, bias=True, residual=True, seed=n)
+        product(hip, ops, m, n, k, F32, bias=True, seed=n)
+
+
 def test_product_refusals(hip, ops):  # noqa: F811
     L, p = ops.lib(), ctypes.c_void_p(16)
 

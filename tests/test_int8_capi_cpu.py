@@ -66,3 +66,21 @@ def test_reference_attention_of_one_key_is_its_value():
     out = b.attention(q)
     value = b.codes[1, b.table[0], :, 0] * b.scales[1, b.table[0]][:, None].astype(np.float64)
     assert np.allclose(out[0], np.repeat(value, 2, 0))
+
+
+def test_rotation_in_place_keeps_its_strides():
+    L, p = capi.lib(), ctypes.c_void_p(16)
+    pa = capi.PaDesc(capi.BF16, capi.BF16, capi.I8, capi.BF16, 4, 2, 64, 32, 10, 3, 1, 40, 0, 0.0, 0, 0)
+
+    def call(q_out=p, **strides):
+        d = capi.RopeAppendDesc(table_dtype=capi.F32, rotary_ndims=64, table_rows=8, table_row_stride=64)
+        for name, value in strides.items():
+            setattr(d, name, value)
+        # (no key pointer: a call whose strides are accepted is refused for that)
+        status = L.hipattn_rope_append(ctypes.byref(pa), ctypes.byref(d), p, None, None, p, p, None, q_out, p, p, p, p, p, p, p, p, None)
+        assert status == capi.INVALID_ARGUMENT
+        return L.hipattn_last_error_string()
+
+    assert b"in place" in call(q_token_stride=512) and b"in place" in call(q_out_head_stride=128, q_out_token_stride=512)
+    assert b"null pointer" in call() and b"null pointer" in call(q_token_stride=512, q_out_token_stride=512)
+    assert b"null pointer" in call(q_token_stride=256) and b"null pointer" in call(q_out=ctypes.c_void_p(32), q_token_stride=512)
