@@ -17,14 +17,22 @@ namespace {
 // 10.1 -> 8.6 us (in tiles 10.7), 16 x 28,672 x 4,096 38.4 -> 33.0 (25.0).
 constexpr int kFewWaves = 8;
 
-template <int kM, int kN>
+template <bool kAligned>
+__device__ __forceinline__ uint4_t piece_at(const int8_t* p) {
+    if constexpr (kAligned) return *(const uint4_t*)p;
+    uint4_t w;
+    __builtin_memcpy(&w, p, 16);
+    return w;
+}
+
+template <int kM, int kN, bool kAligned>
 __global__ __launch_bounds__(64 * kFewWaves) void matmul_i8_few_kernel(MatmulI8Params p) {
     constexpr int kGroup = 4;
     static_assert(kM * kN <= kFewWaves, "a wavefront for each tile of the result");
     __shared__ int4_t sums[kFewWaves][kM * kN][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, row = lane & 15, quarter = lane >> 4;
     const int64_t n0 = 16 * kN * (int64_t)blockIdx.x;
-    const int steps = (int)((p.k + 63) / 64);
+    const int pieces = (int)(p.k / 16), steps = (pieces + 3) / 4;
     const int first = steps * wave / kFewWaves, last = steps * (wave + 1) / kFewWaves;
     const int8_t *w[kN], *x[kM];
 #pragma unroll
@@ -32,7 +40,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void matmul_i8_few_kernel(MatmulI8P
 #pragma unroll
     for (int i = 0; i < kM; i++) x[i] = p.a + min((int64_t)(16 * i + row), p.m - 1) * p.lda + 16 * quarter;
     const bool real = kM > 1 || row < p.m;  // (a single tile: lanes without a row load nothing)
-    const int whole = (int)((p.k - 16 * quarter + 48) / 64);  // steps in which this lane has a piece (k is a multiple of 16)
+    const int whole = (pieces - quarter + 3) / 4;  // steps in which this lane has a piece
     int4_t acc[kN][kM];
 #pragma unroll
     for (int j = 0; j < kN; j++)
@@ -48,7 +56,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void matmul_i8_few_kernel(MatmulI8P
 #pragma unroll
             for (int j = 0; j < kN; j++) {
                 g.w[u][j] = (uint4_t){0u, 0u, 0u, 0u};
-                if (at < whole) g.w[u][j] = *(const uint4_t*)(w[j] + 64 * (int64_t)at);
+                if (at < whole) g.w[u][j] = piece_at<kAligned>(w[j] + 64 * (int64_t)at);
             }
         }
         if (real) {
@@ -57,7 +65,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void matmul_i8_few_kernel(MatmulI8P
                 const int at = min(s + u, last - 1);
 #pragma unroll
                 for (int i = 0; i < kM; i++)
-                    if (at < whole) g.x[u][i] = *(const uint4_t*)(x[i] + 64 * (int64_t)at);
+                    if (at < whole) g.x[u][i] = piece_at<kAligned>(x[i] + 64 * (int64_t)at);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -86,6 +94,19 @@ __global__ __launch_bounds__(64 * kFewWaves) void matmul_i8_few_kernel(MatmulI8P
             multiply(next, s + kGroup);
         }
     }
+    if constexpr (!kAligned) {  // what is left of the rows behind their last whole piece
+        if (wave == kFewWaves - 1 && p.k % 16 != 0) {
+            uint4_t xs[kM];
+#pragma unroll
+            for (int i = 0; i < kM; i++) xs[i] = quarter == 0 ? load_codes16(x[i], 16 * (int64_t)pieces, p.k) : (uint4_t){0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int j = 0; j < kN; j++) {
+                const uint4_t ws = quarter == 0 ? load_codes16(w[j], 16 * (int64_t)pieces, p.k) : (uint4_t){0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int i = 0; i < kM; i++) acc[j][i] = mma_i8_16(ws, xs[i], acc[j][i]);
+            }
+        }
+    }
     // register r: weight row 4 quarter + r, activation row lane % 16 of a tile
 #pragma unroll
     for (int j = 0; j < kN; j++)
@@ -106,15 +127,17 @@ __global__ __launch_bounds__(64 * kFewWaves) void matmul_i8_few_kernel(MatmulI8P
     }
 }
 
-template <int kM, int kN>
+template <int kM, int kN, bool kAligned>
 void launch_few(const MatmulI8Params& p, hipStream_t stream) {
-    hipLaunchKernelGGL((matmul_i8_few_kernel<kM, kN>), dim3((unsigned)((p.n + 16 * kN - 1) / (16 * kN))), dim3(64 * kFewWaves), 0, stream, p);
+    hipLaunchKernelGGL((matmul_i8_few_kernel<kM, kN, kAligned>), dim3((unsigned)((p.n + 16 * kN - 1) / (16 * kN))), dim3(64 * kFewWaves), 0, stream, p);
 }
-void launch_few(const MatmulI8Params& p, bool wide, hipStream_t stream) {
-    if (p.m <= 16)
-        wide ? launch_few<1, 2>(p, stream) : launch_few<1, 1>(p, stream);
+void launch_few(const MatmulI8Params& p, bool wide, bool aligned, hipStream_t stream) {
+    if (!aligned)
+        p.m <= 16 ? launch_few<1, 1, false>(p, stream) : launch_few<2, 1, false>(p, stream);
+    else if (wide)
+        p.m <= 16 ? launch_few<1, 2, true>(p, stream) : launch_few<2, 2, true>(p, stream);
     else
-        wide ? launch_few<2, 2>(p, stream) : launch_few<2, 1>(p, stream);
+        p.m <= 16 ? launch_few<1, 1, true>(p, stream) : launch_few<2, 1, true>(p, stream);
 }
 
 bool float_dtype(int d) { return d == HIPATTN_F32 || d == HIPATTN_F16 || d == HIPATTN_BF16; }
@@ -157,9 +180,10 @@ constexpr TileCost kTileCosts[] = {
     {kI8Tile128Deep, 128, 128, 1 << 30, 5.15f, 0.527f, 0.648f, 0.560f}, {kI8Tile128, 128, 128, 1 << 30, 6.42f, 0.775f, 0.505f, 0.534f},
     {kI8Tile256, 256, 256, 1 << 30, 12.5f, 1.14f, 1.66f, 1.37f},
 };
-// Rows at any address, through registers (us, tiles of 32 rows / 128 rows at their best parts: 64 x 4,095 x 4,095 16.8 / -; 512 x 4,095 x 4,095
+// Rows at any address: up to 32 without LDS (us: 1 x 512 x 2,047 7.1, in tiles 10.5; 1 x 4,096 x 4,095 11.6 and 14.1; 16 x 320 x 1,001 6.5 and 9.9; 16
+// x 4,096 x 4,095 18.2 and 15.5: loads that cross lines), tiles through registers (us, tiles of 32 rows / 128 rows at their best parts: 64 x 4,095 x 4,095 16.8 / -; 512 x 4,095 x 4,095
 // 39.6 / 37.1; 128 x 4,095 x 14,333 38.9 / 34.9; 100 x 2,001 x 1,001 10.4 / 17.8; 8,191 x 6,143 x 4,097 - / 391).
-constexpr TileCost kAnyCosts[] = {{kI8Any32, 32, 128, 512, 3.8f, 0.90f, 0.55f, 0.55f}, {kI8Any128, 128, 128, 1 << 30, 6.5f, 1.65f, 0.94f, 0.94f}};
+constexpr TileCost kAnyCosts[] = {{kI8Any32, 32, 128, 512, 5.63f, 1.12f, 0.746f, 0.763f}, {kI8Any128, 128, 128, 1 << 30, 6.8f, 1.84f, 1.21f, 0.556f}};
 constexpr int kParts[] = {1, 2, 3, 4, 6, 8, 12, 16};
 constexpr float kUnits = 256.0f, kBytesPerUs = 8.0e6f, kSumBytesPerUs = 3.88e6f, kSecondLaunch = 2.88f;
 
@@ -179,12 +203,16 @@ I8Plan plan_of(int64_t m, int64_t n, int64_t k, size_t workspace_bytes, bool ali
             if (us < least) least = us, best = {t.tile, parts};
         }
     };
+    const float steps = (float)k / 2048.0f, rows = (float)m, bytes = (float)n * (float)k;
     if (!aligned) {
+        if (m <= 32) {
+            least = 2.86f + std::max(3.76f * steps * (1.0f + 0.0537f * rows), 3.47f * ceilf((float)n / (16.0f * kUnits)) * steps * (1.0f + 0.0755f * rows));
+            best = {kI8Few, 1};
+        }
         for (const TileCost& t : kAnyCosts) consider(t);
         return best;
     }
     if (m <= 32) {
-        const float steps = (float)k / 2048.0f, rows = (float)m, bytes = (float)n * (float)k;
         const float narrow = 3.88f + std::max({0.808f * steps * (1.0f + 0.0772f * rows), 0.962f * ceilf((float)n / (16.0f * kUnits)) * steps * (1.0f + 0.0527f * rows), bytes / 5.68e6f});
         const float wide = 3.69f + std::max({2.24f * steps * (1.0f + 0.0311f * rows), 1.29f * ceilf((float)n / (32.0f * kUnits)) * steps * (1.0f + 0.0786f * rows), bytes / 5.37e6f});
         least = std::min(narrow, wide);
@@ -218,7 +246,7 @@ hipattn_status matmul_i8(const hipops_matmul_i8_desc* d, const int8_t* a, const 
     const I8Plan plan = plan_of(p.m, p.n, p.k, workspace ? workspace_bytes : 0, aligned);
     hipError_t e = hipSuccess;
     if (plan.tile == kI8Few || plan.tile == kI8FewWide) {
-        launch_few(p, plan.tile == kI8FewWide, stream);
+        launch_few(p, plan.tile == kI8FewWide, aligned, stream);
         e = hipGetLastError();
     } else {
         e = launch_matmul_i8_tiles(p, plan, workspace, stream);

@@ -35,6 +35,25 @@ __device__ __forceinline__ int4_t mma_i8_16(uint4_t a, uint4_t b, int4_t c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int4_t, a), __builtin_bit_cast(int4_t, b), c, 0, 0, 0);
 }
 
+// 16 bytes of a row from `at` on, zeros where it has ended; at any address.
+__device__ __forceinline__ uint4_t load_codes16(const int8_t* row, int64_t at, int64_t k) {
+    uint4_t w = {0u, 0u, 0u, 0u};
+    if (at + 16 <= k) {
+        __builtin_memcpy(&w, row + at, 16);
+    } else if (at < k) {  // (the row's last piece)
+        const int rest = (int)(k - at);
+        unsigned __int128 v = 0;
+        if (k >= 16) {
+            __builtin_memcpy(&v, row + k - 16, 16);
+            v >>= 8 * (16 - rest);
+        } else {
+            for (int e = 0; e < rest; e++) v |= (unsigned __int128)(uint8_t)row[at + e] << (8 * e);
+        }
+        __builtin_memcpy(&w, &v, 16);
+    }
+    return w;
+}
+
 __device__ __forceinline__ float finished(const MatmulI8Params& p, int sum, int64_t i, int64_t j, float b_scale) {
     float x = fmaf((float)sum, (p.a_scales ? p.a_scales[i] : 1.0f) * b_scale, p.bias ? load_scalar(p.bias, j, p.c_dtype) : 0.0f);
     if (p.residual) x += load_scalar(p.residual, i * p.ldc + j, p.c_dtype);

@@ -40,25 +40,6 @@ constexpr int kStageBytes = 128;  // of a row in a stage
 // piece of each) lie on all 64 banks.  (row % 8 instead: 25 times the bank conflicts, 8,192 x 6,144 x 4,096 207 -> 205 us all the same.)
 __device__ __forceinline__ int swizzle(int row) { return (row >> 1) & 7; }
 
-// 16 bytes of a row from `at` on, zeros where it has ended; at any address.
-__device__ __forceinline__ uint4_t load_codes16(const int8_t* row, int64_t at, int64_t k) {
-    uint4_t w = {0u, 0u, 0u, 0u};
-    if (at + 16 <= k) {
-        __builtin_memcpy(&w, row + at, 16);
-    } else if (at < k) {  // (the row's last piece)
-        const int rest = (int)(k - at);
-        unsigned __int128 v = 0;
-        if (k >= 16) {
-            __builtin_memcpy(&v, row + k - 16, 16);
-            v >>= 8 * (16 - rest);
-        } else {
-            for (int e = 0; e < rest; e++) v |= (unsigned __int128)(uint8_t)row[at + e] << (8 * e);
-        }
-        __builtin_memcpy(&w, &v, 16);
-    }
-    return w;
-}
-
 // kBM activation rows x kBN weight rows, kWM x kWN wavefronts, kRing stages of 128 bytes of k.
 // kDirect: rows at multiples of 16 bytes, k too, straight to LDS; otherwise any rows and k, through registers, one stage ahead.
 template <int kBM, int kBN, int kWM, int kWN, int kRing, bool kDirect>

@@ -288,6 +288,15 @@ def test_products_of_few_rows(hip, ops, m):  # noqa: F811
         product(hip, ops, m, n, k, F32, bias=True, seed=n)
 
 
+@pytest.mark.parametrize("m", [1, 7, 16, 17, 32])
+@pytest.mark.parametrize("offset", [0, 3])
+def test_products_of_few_rows_at_any_address(hip, ops, m, offset):  # noqa: F811
+    """Rows that begin anywhere and end inside a piece: k of less than a piece, of whole ones, of a few bytes more in each quarter of a step."""
+    for n, k in ((3, 1), (17, 15), (16, 16), (40, 17), (33, 63), (50, 65), (320, 1001), (100, 2047), (18, 16 * 37 + 9), (4100, 130)):
+        product(hip, ops, m, n, k, BF16, bias=True, residual=True, offset=offset, seed=n)
+        product(hip, ops, m, n, k, F32, pad=(5, 3, 1), offset=offset, extreme=True, seed=n)
+
+
 def test_product_refusals(hip, ops):  # noqa: F811
     L, p = ops.lib(), ctypes.c_void_p(16)
 
