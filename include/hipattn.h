@@ -334,12 +334,12 @@ hipattn_status hipattn_rotate_key_cache(const hipattn_pa_desc* desc, void* key_c
  * Repeating a call changes nothing.  New rows that hold infinities or NaN leave their block's values undefined.
  * 16-bit queries with a head_dim that is a multiple of 8 up to 128, on blocks of 16, 32 or a larger power of two, with at most
  * 16 query heads per kv head or a number that divides into groups of 8 to 16, take the split-context decode kernel (not with
- * alibi_slopes) and, above head size 64, the chunk kernel (with neither alibi_slopes nor sinks).  Other 16-bit calls on power-of-two blocks with
+ * alibi_slopes) and, at head size 128, the chunk kernel (with neither alibi_slopes nor sinks).  Other 16-bit calls on power-of-two blocks with
  * a head_dim that is a multiple of 8 up to 256 take the query-tile kernel, everything else the shape-generic ones.
  * Sequences of 384 new tokens or more have the rows that they attend expanded to fp16 once, in the workspace (at most 256 MiB and
  * 1,024 sequences; hipattn_paged_attention_workspace_size asks for that room where max_context_len bounds it, and a smaller
- * workspace leaves it out).  Rows of several new tokens are attended on fp16 operands: values beyond 65,504 overflow there, and blocks
- * whose largest magnitude is below 1e-3 lose digits (fp16's smallest step is 6e-8); single tokens have no such limits.
+ * workspace leaves it out).  The chunk kernel works on values rounded to fp16: those beyond 65,504 overflow there, and blocks whose
+ * largest magnitude is below 1e-3 lose digits (fp16's smallest step is 6e-8).  The others multiply the codes themselves and have no such limits.
  * The scores output and the cache rotation refuse this type. */
 hipattn_status hipattn_paged_attention_i8(const hipattn_pa_desc* desc, const void* q, const void* k_new, const void* v_new,
                                           void* key_cache, void* value_cache, float* key_scales, float* value_scales,

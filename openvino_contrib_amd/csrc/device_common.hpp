@@ -182,6 +182,16 @@ __device__ __forceinline__ uint4_t dequant8(uint2_t w, half2_t scale, half2_t of
     return r;
 }
 
+// 8 signed codes as the fp16 integers they are
+__device__ __forceinline__ uint4_t codes8_as_half(uint2_t w) {
+    const half2_t bias = {(half_t)1152.0f, (half_t)1152.0f};  // (the sign bit flipped: 1024 + 128 + code)
+    const uint2_t b = w ^ 0x80808080u;
+    uint4_t r;
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = __builtin_bit_cast(uint32_t, biased_half2(b[i >> 1], (i & 1) ? 0x04030402u : 0x04010400u) - bias);
+    return r;
+}
+
 // 8 signed codes -> 8 fp16 values code * scale.  The scale goes in as two fp16 numbers, its rounded value and what that left over:
 // rounded to one, it would be off by the same 2^-12 for every key of a block, which scores of some tens do not average out.
 struct SplitScale {
@@ -192,12 +202,12 @@ __device__ __forceinline__ SplitScale split_scale(float scale) {
     return {half2_t{high, high}, half2_t{low, low}};
 }
 __device__ __forceinline__ uint4_t dequant_codes8(uint2_t w, const SplitScale& s) {
-    const half2_t bias = {(half_t)1152.0f, (half_t)1152.0f};  // (the sign bit flipped: 1024 + 128 + code)
-    const uint2_t b = w ^ 0x80808080u;
+    const uint4_t codes = codes8_as_half(w);
     uint4_t r;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const half2_t c = biased_half2(b[i >> 1], (i & 1) ? 0x04030402u : 0x04010400u) - bias;
+        const uint32_t word = codes[i];  // (a bit cast of a vector's element takes its first)
+        const half2_t c = __builtin_bit_cast(half2_t, word);
         r[i] = __builtin_bit_cast(uint32_t, c * s.high + c * s.low);
     }
     return r;

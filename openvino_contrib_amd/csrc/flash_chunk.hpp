@@ -1307,7 +1307,8 @@ __device__ __forceinline__ void paged_prefill_item(const PagedParams& p, int ind
                 t.block_stride = stride;
                 return t;
             };
-            run_both<false, false, true, 0, false>(in_shadow(t0), in_shadow(t1), lds, p.scale);
+            // (i8: the keys of the copy carry softmax scale and log2(e), so that the queries are not rounded another time)
+            run_both<false, false, true, 0, false>(in_shadow(t0), in_shadow(t1), lds, kI8 ? 1.0f / kLog2e : p.scale);
             return;
         }
     }

@@ -200,7 +200,9 @@ __device__ __forceinline__ uint32_t pack2(int dtype, float lo, float hi) {
 // kU8 (paged, fp16 products): the cache rows are [scale f32][zero-point f32][head_dim bytes]; a piece
 // travels as its eight bytes and the row's scale and zero-point and becomes eight fp16 values
 // (byte - zero-point) * scale on its way into LDS.
-// kI8: rows of head_dim codes, which travel with the scale of their block.
+// kI8: rows of head_dim codes, which travel with the scale of their block.  Codes go to LDS as the fp16 integers they are, the scales
+// as what they do to a key's score and probability: score * scale * key scale * log2(e) + log2(value scale), so that nothing but the
+// probability is rounded, and whatever the scales' size it is bounded; the row sum takes it back by 1 / value scale.
 template <bool kBf16, bool kMask, bool kPaged, int kDP, bool kU8 = false, int kUsed = kDP, bool kI8 = false>
 __device__ __forceinline__ void attend(const Work& w, uint8_t (*lds)[2][tile_bytes<kDP>()]) {
     static_assert(!kI8 || kU8, "i8 caches run the 8-bit form");
@@ -231,7 +233,7 @@ __device__ __forceinline__ void attend(const Work& w, uint8_t (*lds)[2][tile_byt
     // elements 8 (2i + hi) .. + 7 for k-step i, times scale * log2(e)
     vec8 qf[kSteps];
     {
-        const float c = w.scale * kLog2e;
+        const float c = kI8 ? 1.0f : w.scale * kLog2e;  // (i8: a factor of the key's)
         const int row = min(my_row, w.rows - 1);
         const bool q_bf16 = w.q_dtype == HIPATTN_BF16;
 #pragma unroll
@@ -263,6 +265,8 @@ __device__ __forceinline__ void attend(const Work& w, uint8_t (*lds)[2][tile_byt
     // (bad_a, bad_b), a byte per row with the tile in LDS (row_bad), and the softmax masks those keys.
     uint32_t bad_a = 0, bad_b = 0;
     __shared__ uint8_t row_bad[2][kTileK];
+    // kI8, by key: the factor of its scores, log2 of its block's value scale and that scale's inverse
+    __shared__ __attribute__((aligned(16))) float key_factor[2][kI8 ? kTileK : 4], value_log2[2][kI8 ? kTileK : 4], value_inverse[2][kI8 ? kTileK : 4];
     // paged: the block ids of a tile's rows are looked up one tile ahead of its K/V loads, so that
     // those loads do not wait for the table
     int block_of[kPieces];
@@ -324,9 +328,14 @@ __device__ __forceinline__ void attend(const Work& w, uint8_t (*lds)[2][tile_byt
                 if (c == 0) row_bad[buf][r] = (uint8_t)((bad >> s) & 1u);
             }
             if constexpr (kI8) {
-                const auto values = [](const uint4_t& x) { return dequant_codes8((uint2_t){x[0], x[1]}, split_scale(__uint_as_float(x[2]))); };
-                *(uint4_t*)(lds[buf][0] + k_chunk_offset<kDP>(r, c)) = values(stage[s]);
-                *(uint4_t*)(lds[buf][1] + v_chunk_offset<kDP>(r, c)) = values(stage[kPieces + s]);
+                if (c == 0) {
+                    const float value = fmaxf(__uint_as_float(stage[kPieces + s][2]), 0x1p-100f);  // (a block of zeros: too small to count)
+                    key_factor[buf][r] = __uint_as_float(stage[s][2]) * (w.scale * kLog2e);
+                    value_log2[buf][r] = __builtin_amdgcn_logf(value);
+                    value_inverse[buf][r] = 1.0f / value;
+                }
+                *(uint4_t*)(lds[buf][0] + k_chunk_offset<kDP>(r, c)) = codes8_as_half((uint2_t){stage[s][0], stage[s][1]});
+                *(uint4_t*)(lds[buf][1] + v_chunk_offset<kDP>(r, c)) = codes8_as_half((uint2_t){stage[kPieces + s][0], stage[kPieces + s][1]});
             } else if constexpr (kU8) {
                 *(uint4_t*)(lds[buf][0] + k_chunk_offset<kDP>(r, c)) = dequantised8(stage[s]);
                 *(uint4_t*)(lds[buf][1] + v_chunk_offset<kDP>(r, c)) = dequantised8(stage[kPieces + s]);
@@ -431,6 +440,19 @@ __device__ __forceinline__ void attend(const Work& w, uint8_t (*lds)[2][tile_byt
                     for (int e = 0; e < 4; e++) s[mt][4 * g + e] += m4[e];
                 }
         }
+        if constexpr (kI8) {
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const int first = mt * 32 + 8 * g + 4 * hi;  // of four keys
+                    const float4 factor = *(const float4*)&key_factor[buf][first], add = *(const float4*)&value_log2[buf][first];
+                    s[mt][4 * g] = fmaf(s[mt][4 * g], factor.x, add.x);
+                    s[mt][4 * g + 1] = fmaf(s[mt][4 * g + 1], factor.y, add.y);
+                    s[mt][4 * g + 2] = fmaf(s[mt][4 * g + 2], factor.z, add.z);
+                    s[mt][4 * g + 3] = fmaf(s[mt][4 * g + 3], factor.w, add.w);
+                }
+        }
         // ALiBi: slope * (key - query position) joins the score (an exponent to base 2 here).  The slope is
         // fetched where it is used: held across the loop it would cost the larger builds a spilled register.
         if constexpr (kPaged) {
@@ -484,7 +506,12 @@ __device__ __forceinline__ void attend(const Work& w, uint8_t (*lds)[2][tile_byt
                 const float p0 = fast_exp2(s[ks >> 1][(ks & 1) * 8 + 2 * e] - m_use);
                 const float p1 = fast_exp2(s[ks >> 1][(ks & 1) * 8 + 2 * e + 1] - m_use);
                 pw[e] = M::cvt2(p0, p1);
-                sum += p0 + p1;
+                if constexpr (kI8) {  // (register 8 ks' + 2 e of half ks / 2, as above)
+                    const float2 inverse = *(const float2*)&value_inverse[buf][(ks >> 1) * 32 + 16 * (ks & 1) + 8 * (e >> 1) + 4 * hi + 2 * (e & 1)];
+                    sum = fmaf(p0, inverse.x, fmaf(p1, inverse.y, sum));
+                } else {
+                    sum += p0 + p1;
+                }
             }
             pf[ks] = __builtin_bit_cast(vec8, pw);
         }

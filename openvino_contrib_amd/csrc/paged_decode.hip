@@ -158,6 +158,7 @@ __device__ __forceinline__ void expand_blocks_i8(const PagedParams& p, int workg
     uint16_t* const out = (value ? p.shadow_v : p.shadow_k) + (int64_t)index * Hkv * pieces * 16;
     const float* const scales = (value ? p.value_scales : p.key_scales) + (int64_t)(there ? pb : 0) * Hkv;
     const int middle = (Hkv * pieces / 2 + 255) & ~255, last = part & 2 ? Hkv * pieces : min(middle, Hkv * pieces);
+    const float factor = value ? 1.0f : p.scale * kLog2e;  // (keys: what the chunk kernel would give the queries, with a rounding of theirs)
     constexpr int kAtOnce = 4;
     for (int i0 = (part & 2 ? middle : 0) + (int)threadIdx.x; i0 < last; i0 += 256 * kAtOnce) {
         uint4_t w[kAtOnce];
@@ -172,7 +173,7 @@ __device__ __forceinline__ void expand_blocks_i8(const PagedParams& p, int workg
         for (int u = 0; u < kAtOnce; u++) {
             const int i = i0 + 256 * u;
             if (i >= last) break;
-            const SplitScale sc = split_scale(fabsf(scale[u]) < INFINITY ? scale[u] : 0.0f);
+            const SplitScale sc = split_scale(fabsf(scale[u]) < INFINITY ? scale[u] * factor : 0.0f);
             *(uint4_t*)(out + (int64_t)i * 16) = dequant_codes8((uint2_t){w[u][0], w[u][1]}, sc);
             *(uint4_t*)(out + (int64_t)i * 16 + 8) = dequant_codes8((uint2_t){w[u][2], w[u][3]}, sc);
         }

@@ -363,7 +363,7 @@ __device__ __forceinline__ void load_block_i8(BlockRegsI8<kHD>& b, const uint8_t
 struct WaveState {
     float m;          // running max of the scaled scores (log2 domain), per head (lane & 15)
     float l;          // this lane's share of the running sum
-    float corr;       // u8 only: this lane's share of sum_j p'_j zp_j (i8: all of sum_j p'_j)
+    float corr;       // u8 only: this lane's share of sum_j p'_j zp_j
     float4_t acc[8];  // acc[e][r] = O[head][(kg*4 + r)*8 + e]; i8 at head size 64: e < 4, O[head][(kg*4 + r)*4 + e]
 };
 
@@ -522,16 +522,18 @@ __device__ __forceinline__ void process_block(WaveState& st, BlockRegs<kU8>& b, 
 }
 
 
-// A unit of an i8 cache.  Codes become the exact fp16 integers 1024 + 128 + code (the sign bit flipped, then as the u8 bytes), so
-// that scores are off by 1152 sum(q) and outputs by 1152 sum(p): one constant per head, taken out of the scores here and of
-// the outputs when the segment is done.  A tile is one block's, so its two scales are one number each:
+// A unit of an i8 cache.  Codes become the exact fp16 integers 1024 + 128 + code (the sign bit flipped, then as the u8 bytes).  The keys'
+// stay so, and scores are off by 1152 sum(q), one constant per head that is taken out here; the values' lose their 1152 by a packed
+// subtraction, for outputs that carry 1152 sum(p) along through a context of thousands of tokens lose two digits of fp32 to it (fp16
+// results of 64 sequences of up to 8,192 tokens were 3.1e-4 off fp64 instead of 2.5e-4, their own rounding 2.1e-4 of it).  A tile is one
+// block's, so its two scales are one number each:
 //   score * log2(e) = (s - 1152 sum(q)) key,  key = key scale * softmax scale * log2(e)
 //   v_scale exp2(score - reference) = exp2(score + log2(v_scale) - reference)
 // The value scale joins the exponent: the running maximum then bounds what is multiplied with the codes, in fp16 whatever the
 // scales' size, and the row sum takes the probabilities back by 1 / v_scale.  (A u8 row's scale and zero-point cost the u8 form
 // two broadcasts and two more operations for every probability.)
-// sum(p), of the probabilities as they are rounded for the product, is one more product, with ones.  (The row sum takes the unrounded
-// ones: next to a block of large values, those of a block of small ones may round to nothing and still count as weight.)
+// The row sum takes the unrounded probabilities: next to a block of large values, those of a block of small ones may round to nothing
+// and still count as weight.
 // A unit costs 241 vector instructions at head size 128, all around it included; with a comparison for every score and sums of the rounded
 // probabilities lane by lane it was 334 (304 at head size 64, with eight columns of V to a lane).  64 sequences of 512 to 8,192 tokens,
 // 32 heads on 8, blocks of 32, the whole call: head size 64 68.2 us (79.7 before; their bytes take 47.8 at 5.9 TB/s), 128 117.3 (119.4;
@@ -592,18 +594,19 @@ __device__ __forceinline__ void process_block_i8(WaveState& st, const BlockRegsI
 #pragma unroll
         for (int e = 0; e < kOut; e++) st.acc[e] *= alpha;
     }
-    const half8_t ones = as_half8((uint4_t){0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u});
-    const float4_t sums = Op::mma(ones, pf, (float4_t){0.f, 0.f, 0.f, 0.f});
+    const half2_t bias = {(half_t)kCodeBias, (half_t)kCodeBias};
 #pragma unroll
     for (int e = 0; e < kOut; e++) {
         uint4_t w;
         const uint32_t sel = 0x0c000c00u | ((4u + (e & 3)) << 16) | (uint32_t)(e & 3);
 #pragma unroll
-        for (int jp = 0; jp < 4; jp++) w[jp] = __builtin_amdgcn_perm(b.v[2 * jp + 1][e >> 2], b.v[2 * jp][e >> 2], sel) ^ 0x64806480u;
+        for (int jp = 0; jp < 4; jp++) {
+            const uint32_t biased = __builtin_amdgcn_perm(b.v[2 * jp + 1][e >> 2], b.v[2 * jp][e >> 2], sel) ^ 0x64806480u;
+            w[jp] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, biased) - bias);
+        }
         st.acc[e] = Op::mma(Op::from_bits(w), pf, st.acc[e]);
     }
     st.l = st.l * alpha + fmaf(lsum[0], u.value_inverse[0], lsum[1] * u.value_inverse[1]);
-    st.corr = st.corr * alpha + sums[0];
 }
 
 // Length of one (sequence, kv head) segment on the work line: its blocks plus `switch_cost`
@@ -1153,9 +1156,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams& p, const Kv
         float l = st.l, corr = st.corr;
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
-        if constexpr (kI8) {
-            corr *= kCodeBias;
-        } else if constexpr (kU8) {
+        if constexpr (kU8 && !kI8) {
             corr += __shfl_xor(corr, 16, 64);
             corr += __shfl_xor(corr, 32, 64);
         }
@@ -1170,7 +1171,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedParams& p, const Kv
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     float v = kRows == 4 ? st.acc[e][r] : st.acc[e & 3][2 * r + (e >> 2)];
-                    if constexpr (kU8) v -= corr;
+                    if constexpr (kU8 && !kI8) v -= corr;
                     o[e] = v * inv;
                 }
                 const int d0 = (kg * kRows + r) * 8;
