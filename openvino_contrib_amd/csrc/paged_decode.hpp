@@ -534,10 +534,10 @@ __device__ __forceinline__ void process_block(WaveState& st, BlockRegs<kU8>& b, 
 // two broadcasts and two more operations for every probability.)
 // The row sum takes the unrounded probabilities: next to a block of large values, those of a block of small ones may round to nothing
 // and still count as weight.
-// A unit costs 241 vector instructions at head size 128, all around it included; with a comparison for every score and sums of the rounded
+// A unit costs 266 vector instructions at head size 128, all around it included; with a comparison for every score and sums of the rounded
 // probabilities lane by lane it was 334 (304 at head size 64, with eight columns of V to a lane).  64 sequences of 512 to 8,192 tokens,
-// 32 heads on 8, blocks of 32, the whole call: head size 64 68.2 us (79.7 before; their bytes take 47.8 at 5.9 TB/s), 128 117.3 (119.4;
-// 95.5), 80 (padded) 89.1 (112; 59.7).
+// 32 heads on 8, blocks of 32, the whole call: head size 64 68.3 us (79.7 before; their bytes take 47.8 at 5.9 TB/s), 128 116.2 (119.4;
+// 95.5), 80 (padded) 86.6 (112; 59.7).
 constexpr float kCodeBias = kByteBias + 128.0f;
 template <int kHD, bool kTileMask>
 __device__ __forceinline__ void process_block_i8(WaveState& st, const BlockRegsI8<kHD>& b, const half8_t (&qf)[4], float sumq, const UnitScales& u,
