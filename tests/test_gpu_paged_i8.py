@@ -212,6 +212,26 @@ def test_new_prompts_are_expanded_once(hip, bs):
             check(hip, b, bound_of(True, F16, F32, True), out_dtype=F32, window=1500, bound_len=0)
 
 
+@pytest.mark.parametrize("D", [8, 40, 72, 136, 192, 248, 256])
+@pytest.mark.parametrize("bs", [8, 32, 64])
+def test_query_tiles_at_other_head_sizes(hip, D, bs):
+    b = R.Batch(15, [(0, 70), (300, 1), (33, 129), (0, 2), (500, 64)], 4, 2, D, bs)
+    check(hip, b, bound_of(True, F16, F32, True), out_dtype=F32)
+    check(hip, b, bound_of(True, BF16, BF16, True), q_dtype=BF16, window=90)
+
+
+@pytest.mark.parametrize("factor", [1e-8, 1e-4, 1e6])
+@pytest.mark.parametrize("D,seqs", [(128, [(40, 1), (700, 1), (31, 1)]), (64, [(40, 1), (700, 1)]), (64, [(0, 70), (300, 30)]), (192, [(0, 50), (100, 1)])])
+def test_values_beyond_the_range_of_16_bits(hip, D, seqs, factor):
+    """Codes are multiplied as they are and their scale joins in fp32, in the decode and the query-tile kernels: results are as close to fp64,
+    relative to their size, as at any other magnitude (probabilities rounded to fp16: the bound of the fp16 results)."""
+    b = R.Batch(16, seqs, 8, 2, D, 32)
+    b.scales[1] *= np.float32(factor)
+    got, q, _, path = run(hip, b, out_dtype=F32)
+    ref = b.attention(q)
+    assert np.max(np.abs(got - ref)) <= 2e-3 * np.abs(ref).max(), path
+
+
 def test_refusals(hip):
     L, p = hip.lib(), ctypes.c_void_p(16)
     pa = hip.PaDesc(BF16, BF16, I8, BF16, 8, 2, 128, 32, 100, 4, 2, 64, 0, 0.0, 0, 0)
