@@ -192,23 +192,17 @@ __device__ __forceinline__ uint4_t codes8_as_half(uint2_t w) {
     return r;
 }
 
-// 8 signed codes -> 8 fp16 values code * scale.  The scale goes in as two fp16 numbers, its rounded value and what that left over:
-// rounded to one, it would be off by the same 2^-12 for every key of a block, which scores of some tens do not average out.
-struct SplitScale {
-    half2_t high, low;
-};
-__device__ __forceinline__ SplitScale split_scale(float scale) {
-    const half_t high = (half_t)scale, low = (half_t)(scale - (float)high);
-    return {half2_t{high, high}, half2_t{low, low}};
-}
-__device__ __forceinline__ uint4_t dequant_codes8(uint2_t w, const SplitScale& s) {
+// 8 signed codes -> the fp16 numbers nearest to code * scale.  The scale stays in fp32: as fp16 it would be off by the same amount for every
+// key of a block, which scores of some tens do not average out, and small ones would have few digits or none.
+__device__ __forceinline__ uint4_t dequant_codes8(uint2_t w, float scale) {
     const uint4_t codes = codes8_as_half(w);
     uint4_t r;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const uint32_t word = codes[i];  // (a bit cast of a vector's element takes its first)
         const half2_t c = __builtin_bit_cast(half2_t, word);
-        r[i] = __builtin_bit_cast(uint32_t, c * s.high + c * s.low);
+        const half2_t y = {(half_t)fmaf((float)c[0], scale, 0.0f), (half_t)fmaf((float)c[1], scale, 0.0f)};
+        r[i] = __builtin_bit_cast(uint32_t, y);
     }
     return r;
 }

@@ -874,7 +874,7 @@ __device__ __forceinline__ void run_pair(const Tile& t, int kv_lo, int kv_hi, ui
             lds_uint4* const lo = (lds_uint4*)(rowp + (((2 * u8_piece) ^ (u8_row & 15)) << 4));
             lds_uint4* const hi8 = (lds_uint4*)(rowp + (((2 * u8_piece + 1) ^ (u8_row & 15)) << 4));
             if constexpr (kI8) {  // (softmax scale and log2(e) on the keys instead of the queries: one rounding of the product less)
-                const SplitScale sc = split_scale(x.k_sz.x * c);
+                const float sc = x.k_sz.x * c;
                 *lo = dequant_codes8(x.k_lo, sc);
                 *hi8 = dequant_codes8(x.k_hi, sc);
             } else {
@@ -890,7 +890,7 @@ __device__ __forceinline__ void run_pair(const Tile& t, int kv_lo, int kv_hi, ui
             lds_uint4* const lo = (lds_uint4*)(rowp + (((2 * u8_piece) ^ (4 * (u8_row & 3))) << 4));
             lds_uint4* const hi8 = (lds_uint4*)(rowp + (((2 * u8_piece + 1) ^ (4 * (u8_row & 3))) << 4));
             if constexpr (kI8) {
-                const SplitScale sc = split_scale(x.v_sz.x);
+                const float sc = x.v_sz.x;
                 *lo = dequant_codes8(x.v_lo, sc);
                 *hi8 = dequant_codes8(x.v_hi, sc);
             } else {

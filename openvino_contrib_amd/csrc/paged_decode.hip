@@ -173,7 +173,7 @@ __device__ __forceinline__ void expand_blocks_i8(const PagedParams& p, int workg
         for (int u = 0; u < kAtOnce; u++) {
             const int i = i0 + 256 * u;
             if (i >= last) break;
-            const SplitScale sc = split_scale(fabsf(scale[u]) < INFINITY ? scale[u] * factor : 0.0f);
+            const float sc = fabsf(scale[u]) < INFINITY ? scale[u] * factor : 0.0f;
             *(uint4_t*)(out + (int64_t)i * 16) = dequant_codes8((uint2_t){w[u][0], w[u][1]}, sc);
             *(uint4_t*)(out + (int64_t)i * 16 + 8) = dequant_codes8((uint2_t){w[u][2], w[u][3]}, sc);
         }

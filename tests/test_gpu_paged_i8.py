@@ -253,3 +253,45 @@ def test_refusals(hip):
     score = ctypes.c_void_p(16)
     assert L.hipattn_paged_attention_scores(ctypes.byref(pa), p, p, p, p, p, p, None, score, 10, p, 1 << 20, None) == hip.UNSUPPORTED
     assert L.hipattn_rotate_key_cache(ctypes.byref(pa), p, p, 1, p, 1, p, F32, 4, None) == hip.UNSUPPORTED
+
+
+class ScaledNormal:
+    """Draws of N(0, 1) times a factor, for a batch's queries."""
+
+    def __init__(self, rng, factor):
+        self.rng, self.factor = rng, factor
+
+    def standard_normal(self, shape):
+        return self.rng.standard_normal(shape) * self.factor
+
+
+CHUNKS = [[(0, 70), (300, 30), (90, 1)], [(0, 450), (200, 400), (90, 1)]]  # rows converted tile by tile; expanded once, ahead of the kernel
+
+
+@pytest.mark.parametrize("factor", [1.0, 1e-2, 1e-3, 1e-4, 1e-5, 1e-6])
+@pytest.mark.parametrize("bs", [16, 32])
+@pytest.mark.parametrize("seqs", CHUNKS)
+def test_chunks_of_small_values(hip, seqs, bs, factor):
+    """The chunk kernel's values are the fp16 numbers nearest to code * scale.  Off fp64, relative to the largest result: 2^-11 for the value,
+    2^-11 for the probability and 2^-11 for the sum that divides it, some 2e-4 from the keys' roundings: below 2e-3; and half of fp16's
+    smallest step, 2^-25, whatever the size."""
+    b = R.Batch(17, seqs, 8, 2, 128, bs)
+    b.scales[1] *= np.float32(factor)
+    got, q, _, path = run(hip, b, out_dtype=F32)
+    ref = b.attention(q)
+    assert np.max(np.abs(got - ref)) <= 2e-3 * np.abs(ref).max() + 2.0 ** -25, path
+
+
+@pytest.mark.parametrize("factor", [1.0, 1e-1, 1e-2, 1e-3])
+@pytest.mark.parametrize("bs", [16, 32])
+@pytest.mark.parametrize("seqs", CHUNKS)
+def test_chunks_of_small_keys(hip, seqs, bs, factor):
+    """Small keys under large queries, scores as at any other size.  A score is a sum of 128 products of keys that are each rounded to fp16 (rms
+    1.7e-4 of it, also at 1e-3, where the smaller ones lie among fp16's last steps): 2.4e-4 rms in units of the exponent, 8e-4 of a weight
+    at four and a half times that, twice for two keys; with the three roundings of 2^-11 below 4e-3 of the largest result."""
+    b = R.Batch(18, seqs, 8, 2, 128, bs)
+    b.scales[0] *= np.float32(factor)
+    b.rng = ScaledNormal(b.rng, 1 / factor)
+    got, q, _, path = run(hip, b, out_dtype=F32)
+    ref = b.attention(q)
+    assert np.max(np.abs(got - ref)) <= 4e-3 * np.abs(ref).max(), path
