@@ -339,9 +339,9 @@ hipattn_status hipattn_rotate_key_cache(const hipattn_pa_desc* desc, void* key_c
  * Sequences of 384 new tokens or more have the rows that they attend expanded to fp16 once, in the workspace (at most 256 MiB and
  * 1,024 sequences; hipattn_paged_attention_workspace_size asks for that room where max_context_len bounds it, and a smaller
  * workspace leaves it out).  The chunk kernel works on the fp16 numbers nearest to code * scale (keys: times softmax scale and log2(e) as
- * well): those beyond 65,504 overflow there, and below 6.1e-5 they lie 6e-8 apart, which the results of a block of values notice from a
- * largest magnitude of about 1e-4 on downwards (1e-5: 0.3 % of it; keys add 3e-8 times the query's magnitude to a score, whatever their
- * own).  The other kernels multiply the codes themselves and have no such limits.
+ * well).  A block with larger ones than 65,504 is scaled down to that there; below 6.1e-5 they lie 6e-8 apart, which the results of a
+ * block of values notice from a largest magnitude of about 1e-4 on downwards (1e-5: 0.3 % of it; keys add 3e-8 times the query's
+ * magnitude to a score, whatever their own).  The other kernels multiply the codes themselves and have no such limits.
  * The scores output and the cache rotation refuse this type. */
 hipattn_status hipattn_paged_attention_i8(const hipattn_pa_desc* desc, const void* q, const void* k_new, const void* v_new,
                                           void* key_cache, void* value_cache, float* key_scales, float* value_scales,

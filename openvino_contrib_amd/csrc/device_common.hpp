@@ -192,16 +192,21 @@ __device__ __forceinline__ uint4_t codes8_as_half(uint2_t w) {
     return r;
 }
 
+// The largest scale whose codes (up to 127) stay finite in fp16; NaN becomes it too.
+__device__ __forceinline__ float scale_within_half(float scale) { return fminf(scale, 65504.0f / 127.0f); }
+
 // 8 signed codes -> the fp16 numbers nearest to code * scale.  The scale stays in fp32: as fp16 it would be off by the same amount for every
-// key of a block, which scores of some tens do not average out, and small ones would have few digits or none.
+// key of a block, which scores of some tens do not average out, and small ones would have few digits or none.  One fused operation a code takes
+// the bias of codes8_as_half off as well: 1152 times a scale of 20 bits is exact in fp32 (so is the sum then), and the last four bits of
+// a scale are 2^-20 of it.
 __device__ __forceinline__ uint4_t dequant_codes8(uint2_t w, float scale) {
-    const uint4_t codes = codes8_as_half(w);
+    const float s = __uint_as_float(__float_as_uint(scale) & 0xfffffff0u), off = -1152.0f * s;
+    const uint2_t b = w ^ 0x80808080u;
     uint4_t r;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const uint32_t word = codes[i];  // (a bit cast of a vector's element takes its first)
-        const half2_t c = __builtin_bit_cast(half2_t, word);
-        const half2_t y = {(half_t)fmaf((float)c[0], scale, 0.0f), (half_t)fmaf((float)c[1], scale, 0.0f)};
+        const half2_t c = biased_half2(b[i >> 1], (i & 1) ? 0x04030402u : 0x04010400u);
+        const half2_t y = {(half_t)fmaf((float)c[0], s, off), (half_t)fmaf((float)c[1], s, off)};
         r[i] = __builtin_bit_cast(uint32_t, y);
     }
     return r;

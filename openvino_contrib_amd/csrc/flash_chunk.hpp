@@ -620,7 +620,7 @@ __device__ __forceinline__ void barrier_keeping_loads(int keep) {  // keep is ev
 // ever meets the zeros the query fragments hold in those columns, or lands in output columns that
 // are not stored.
 template <bool kBf16, bool kU8 = false, bool kPaged = true, int kMask = 0, bool kPad = false, bool kI8 = false>
-__device__ __forceinline__ void run_pair(const Tile& t, int kv_lo, int kv_hi, uint8_t* lds_generic, float scale) {
+__device__ __forceinline__ void run_pair(const Tile& t, int kv_lo, int kv_hi, int first_key, uint8_t* lds_generic, float scale) {
     static_assert(kPaged || !kU8, "dense K/V are 16-bit");
     static_assert(!kPad || !kU8, "smaller head sizes: 16-bit K/V");
     const int grow = kPad ? 2 * t.head_dim : kRowBytes;  // bytes from row to row in memory
@@ -814,8 +814,8 @@ __device__ __forceinline__ void run_pair(const Tile& t, int kv_lo, int kv_hi, ui
     const int u8_row = 8 * wave + (lane >> 3), u8_piece = lane & 7;
     // address of this lane's row of tile j (entry: the block table entry of the wavefront's rows)
     constexpr int kByteRow = kI8 ? kD : kU8RowBytes;
-    // (and kI8: the block's scale.  What a block outside the cache, or one that no key of the tile is attended in, may hold
-    // beside codes that are never used -- infinities, NaN -- becomes zero, as its probabilities would not make it that.)
+    // (and kI8: the block's scale.  A block outside the cache, and one that lies ahead of the first key that anything of the workgroup's
+    // attends, may hold any codes beside any scale, which times a probability of zero is not always zero: its values are made zeros.)
     auto u8_row_address = [&](const uint8_t* base, int j, int entry, const float* scales, float& scale) __attribute__((always_inline)) -> const uint8_t* {
         const int key0 = kv_lo + j * kTileK + 8 * wave;
         int key = kv_lo + j * kTileK + u8_row;
@@ -829,7 +829,8 @@ __device__ __forceinline__ void run_pair(const Tile& t, int kv_lo, int kv_hi, ui
         const int inside = min(max(pb, 0), t.num_blocks - 1);
         if constexpr (kI8) {
             scale = scales[(int64_t)inside * t.scale_stride];
-            scale = inside == pb && fabsf(scale) < INFINITY ? scale : 0.0f;
+            const bool ahead = (key0 | (t.block_size - 1)) < first_key;  // (wave-uniform: eight rows of one block)
+            scale = inside == pb && !ahead ? scale : 0.0f;
         }
         return base + (int64_t)inside * t.block_stride + (int64_t)(key & (t.block_size - 1)) * kByteRow;
     };
@@ -874,7 +875,7 @@ __device__ __forceinline__ void run_pair(const Tile& t, int kv_lo, int kv_hi, ui
             lds_uint4* const lo = (lds_uint4*)(rowp + (((2 * u8_piece) ^ (u8_row & 15)) << 4));
             lds_uint4* const hi8 = (lds_uint4*)(rowp + (((2 * u8_piece + 1) ^ (u8_row & 15)) << 4));
             if constexpr (kI8) {  // (softmax scale and log2(e) on the keys instead of the queries: one rounding of the product less)
-                const float sc = x.k_sz.x * c;
+                const float sc = scale_within_half(x.k_sz.x * c);
                 *lo = dequant_codes8(x.k_lo, sc);
                 *hi8 = dequant_codes8(x.k_hi, sc);
             } else {
@@ -890,7 +891,7 @@ __device__ __forceinline__ void run_pair(const Tile& t, int kv_lo, int kv_hi, ui
             lds_uint4* const lo = (lds_uint4*)(rowp + (((2 * u8_piece) ^ (4 * (u8_row & 3))) << 4));
             lds_uint4* const hi8 = (lds_uint4*)(rowp + (((2 * u8_piece + 1) ^ (4 * (u8_row & 3))) << 4));
             if constexpr (kI8) {
-                const float sc = x.v_sz.x;
+                const float sc = scale_within_half(x.v_sz.x);
                 *lo = dequant_codes8(x.v_lo, sc);
                 *hi8 = dequant_codes8(x.v_hi, sc);
             } else {
@@ -1192,7 +1193,9 @@ __device__ __forceinline__ void run_both(const Tile& t0, const Tile& t1, uint8_t
         kv_hi = max(hi0, hi1);
     }
     const int group = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8);
-    run_pair<kBf16, kU8, kPaged, kMask, kPad, kI8>(group ? t1 : t0, kv_lo, kv_hi, lds, scale);
+    // (t0's window begins first; kv_lo is that rounded down to whole tiles)
+    const int first_key = kI8 && t0.window > 0 ? max(0, t0.pos0 - t0.window + 1) : 0;
+    run_pair<kBf16, kU8, kPaged, kMask, kPad, kI8>(group ? t1 : t0, kv_lo, kv_hi, first_key, lds, scale);
 }
 
 // One workgroup per (128-row query tile of a multi-token sequence, pair of query heads) or, with an

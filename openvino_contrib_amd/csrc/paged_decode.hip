@@ -151,6 +151,9 @@ __device__ __forceinline__ void expand_blocks_i8(const PagedParams& p, int workg
     const int pb = p.block_indices[p.block_indices_begins[owner] + first + (index - base)];
     const bool there = pb >= 0 && pb < p.num_blocks;
     if (part == 0 && threadIdx.x == 0) p.shadow_table[index] = there ? index - base : -1;
+    // (a block of the first tile that ends ahead of the window may hold anything: zeros, as in the chunk kernel)
+    const int window_begin = p.sliding_window > 0 ? max(0, p.past_lens[owner] - p.sliding_window + 1) : 0;
+    const bool attended = there && (first + (index - base) + 1) * p.block_size > window_begin;
     const int Hkv = p.num_heads_kv / p.kv_share;
     const int pieces = p.block_size * 8, shift = __builtin_ctz(pieces);  // sixteen codes each, of a head's rows
     const bool value = part & 1;
@@ -167,13 +170,13 @@ __device__ __forceinline__ void expand_blocks_i8(const PagedParams& p, int workg
         for (int u = 0; u < kAtOnce; u++) {
             const int i = min(i0 + 256 * u, last - 1);
             w[u] = *(const uint4_t*)(codes + (int64_t)i * 16);
-            scale[u] = there ? scales[i >> shift] : 0.0f;
+            scale[u] = attended ? scales[i >> shift] : 0.0f;
         }
 #pragma unroll
         for (int u = 0; u < kAtOnce; u++) {
             const int i = i0 + 256 * u;
             if (i >= last) break;
-            const float sc = fabsf(scale[u]) < INFINITY ? scale[u] * factor : 0.0f;
+            const float sc = scale_within_half(scale[u] * factor);
             *(uint4_t*)(out + (int64_t)i * 16) = dequant_codes8((uint2_t){w[u][0], w[u][1]}, sc);
             *(uint4_t*)(out + (int64_t)i * 16 + 8) = dequant_codes8((uint2_t){w[u][2], w[u][3]}, sc);
         }

@@ -295,3 +295,33 @@ def test_chunks_of_small_keys(hip, seqs, bs, factor):
     got, q, _, path = run(hip, b, out_dtype=F32)
     ref = b.attention(q)
     assert np.max(np.abs(got - ref)) <= 4e-3 * np.abs(ref).max(), path
+
+
+@pytest.mark.parametrize("scale", [1000.0, 1e20, 3e38, -1e20, -600.0, np.inf, np.nan])
+@pytest.mark.parametrize("bs", [16, 32])
+@pytest.mark.parametrize("D,new", [(128, 30), (128, 400), (128, 1), (64, 30)])
+def test_blocks_ahead_of_the_window_may_have_any_scale(hip, D, new, bs, scale):
+    """Blocks that the window has left, in the first 64 keys that a kernel looks at, with whatever codes and scales their next owner put there."""
+    past, window = 330, 40
+    b = R.Batch(19, [(past, new), (0, 3)], 4, 2, D, bs)
+    for e in range((past - window + 1) // bs):
+        block = b.table[b.table_begins[0] + e]
+        b.scales[:, block] = scale
+        b.codes[:, block, :, ::3], b.codes[:, block, :, 1::3], b.codes[:, block, :, 2::3] = -128, 0, 127
+    got, q, _, path = run(hip, b, out_dtype=F32, window=window)
+    ref = b.attention(q, window)
+    assert np.isfinite(got).all(), path
+    assert scaled_bound_error(got, ref, path) <= 1e-2
+
+
+@pytest.mark.parametrize("seqs", CHUNKS)
+def test_values_up_to_the_largest_of_16_bits(hip, seqs):
+    """Chunks of values up to 65,504 are attended as any others; larger ones are cut to that in a block, and stay finite."""
+    b = R.Batch(20, seqs, 8, 2, 128, 32)
+    b.scales[1] = np.float32(65504 / 127)
+    got, q, _, path = run(hip, b, out_dtype=F32)
+    ref = b.attention(q)
+    assert np.max(np.abs(got - ref)) <= 2e-3 * np.abs(ref).max(), path
+    b.scales[1] *= 4
+    got, q, _, path = run(hip, b, out_dtype=F32)
+    assert np.isfinite(got).all(), path
