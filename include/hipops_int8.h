@@ -19,7 +19,7 @@ extern "C" {
  * codes[r, i] = clamp(rint(y[r, i] * (1 / scales[r])), -127, 127), scales[r] = max_i |y[r, i]| * (1 / 127), all in fp32; a scale
  * below 1e-30 is 0, and so are its codes.  y is one of
  *   HIPOPS_QUANTIZE_PLAIN      x[r, i]
- *   HIPOPS_QUANTIZE_RMS_NORM   x[r, i] * 1/sqrt(mean_i(x[r, i]^2) + eps) * gamma[i]   (gamma [width], or NULL: ones)
+ *   HIPOPS_QUANTIZE_RMS_NORM   x[r, i] * 1/sqrt(mean_i(x[r, i]^2) + eps) * gamma[i]   (gamma [width], or NULL: ones; zeros where the root is of 0)
  *   HIPOPS_QUANTIZE_GLU        act(x[r, g + i]) * x[r, u + i], rows of x 2 * width long, as hipops_glu
  * in fp32, not rounded in between.  x_row_stride: elements between rows of x (0: packed); codes [rows, width] and scales [rows]
  * are packed.  A row that holds infinities or NaN has undefined codes and scale; other rows are not touched by it. */

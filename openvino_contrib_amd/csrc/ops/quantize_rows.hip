@@ -32,6 +32,12 @@ __device__ __forceinline__ float scale_of_peak(float peak) {
 }
 __device__ __forceinline__ int code_of(float y, float inverse) { return (int)fminf(fmaxf(rintf(y * inverse), -127.0f), 127.0f); }
 
+// 1 / rms of a row with this sum of squares; 0 where mean square and eps are both 0, so that a row of zeros stays one (and not 0 times infinity)
+__device__ __forceinline__ float inverse_rms(const QuantizeParams& p, float sq) {
+    const float square = sq / (float)p.width + p.eps;
+    return square == 0.0f ? 0.0f : 1.0f / sqrtf(square);
+}
+
 // over all lanes of the workgroup; `partial` is free again after the next barrier
 template <bool kMax>
 __device__ __forceinline__ float reduce(float x, float* partial) {
@@ -141,7 +147,7 @@ __device__ __forceinline__ void quantize_row(const QuantizeParams& p, int64_t ro
 #pragma unroll
         for (int e = 0; e < 8; e++) peak = fmaxf(peak, fabsf(y[c].v[e]));
     over(sq, peak);
-    const float inv = kSource == HIPOPS_QUANTIZE_RMS_NORM ? 1.0f / sqrtf(sq / (float)p.width + p.eps) : 1.0f;
+    const float inv = kSource == HIPOPS_QUANTIZE_RMS_NORM ? inverse_rms(p, sq) : 1.0f;
     const float scale = scale_of_peak(peak * inv);
     const float inverse = scale > 0.0f ? inv * (1.0f / scale) : 0.0f;
     if (lane == 0) p.scales[row] = scale;
@@ -202,7 +208,7 @@ __global__ __launch_bounds__(256) void quantize_rows_scalar_kernel(QuantizeParam
             const float x = value1<kSource>(p, at, i);
             sq = fmaf(x, x, sq);
         }
-        inv = 1.0f / sqrtf(reduce<false>(sq, sums) / (float)p.width + p.eps);
+        inv = inverse_rms(p, reduce<false>(sq, sums));
     }
     const auto value = [&](int64_t i) {
         float y = value1<kSource>(p, at, i);

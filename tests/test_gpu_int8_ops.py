@@ -314,3 +314,17 @@ def test_product_refusals(hip, ops):  # noqa: F811
     n = ctypes.c_size_t(0)
     assert L.hipops_matmul_i8_workspace_size(ctypes.byref(ops.MatmulI8Desc(BF16, 4, 64, 131072, 0, 0, 0)), ctypes.byref(n)) == hip.UNSUPPORTED
     assert L.hipops_matmul_i8_workspace_size(ctypes.byref(ops.MatmulI8Desc(BF16, 4, 64, 64, 0, 0, 0)), None) == hip.INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("gamma", [False, True])
+@pytest.mark.parametrize("rows,width", [(3, 64), (5, 4096), (4, 14336), (1500, 512), (4, 37), (2, 33000)])
+def test_rows_of_zeros_without_an_epsilon(hip, ops, rows, width, gamma, dtype):  # noqa: F811
+    """A row whose mean square and eps are both 0 has scale 0 and codes 0, in every form of the kernel; its neighbours are what they are alone."""
+    x = np.random.default_rng(width).standard_normal((rows, width)).astype(np.float32)
+    x[1::2] = 0
+    g = np.random.default_rng(1).standard_normal(width) if gamma else None
+    codes, scales, exact, gv = quantised(hip, ops, x, dtype, 1, g, dtype, eps=0.0)
+    assert not codes[1::2].any() and np.array_equal(scales[1::2], np.zeros(len(scales[1::2]), np.float32))
+    e = exact[::2].astype(np.float64)
+    near(codes[::2], scales[::2], e / np.sqrt((e ** 2).mean(1, keepdims=True)) * np.asarray(gv, np.float64))
