@@ -359,7 +359,8 @@ hipattn_status hipattn_paged_attention_i8(const hipattn_pa_desc* desc, const voi
  * fp32, each rounded by itself, and are rounded once more to the type of q_out or stored in the cache straight from
  * fp32 -- converted, or quantised (HIPATTN_U8 as by hipattn_kv_cache_write, HIPATTN_I8 as described at hipattn_paged_attention_i8).  Values
  * are stored as they are.  Tokens whose row lies outside [0, table_rows), and tokens outside every sequence, are not turned;
- * tokens whose cache position has no block are not stored, as in hipattn_paged_attention.
+ * tokens whose cache position has no block are not stored, as in hipattn_paged_attention.  With num_seqs == 0 the
+ * queries are copied as they are, and of the pointers only q and q_out are used.
  *
  * q, k_new, v_new, q_out: element i of head h of token t at t * token_stride + h * head_stride + i, in elements; a stride of 0
  * stands for packed rows (head_stride = head_dim, token_stride = heads * head_dim), so the three may be slices of one

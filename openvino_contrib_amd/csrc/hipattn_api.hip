@@ -531,10 +531,12 @@ HIPATTN_EXPORT hipattn_status hipattn_rope_append(const hipattn_pa_desc* desc, c
     if (q && q == q_out && (q_head != out_head || q_token != out_token))
         return fail(HIPATTN_INVALID_ARGUMENT, "rope_append: in place with rows %lld, %lld apart and %lld, %lld afterwards", (long long)q_token, (long long)q_head,
                     (long long)out_token, (long long)out_head);
-    if (desc->num_tokens == 0 || desc->num_seqs == 0) return HIPATTN_OK;
-    if (!k_new || !v_new || !key_cache || !value_cache || !past_lens || !subsequence_begins || !block_indices || !block_indices_begins)
+    // (no sequences: every token is outside them all, and its queries are copied as they are)
+    if (desc->num_tokens == 0 || (desc->num_seqs == 0 && q == q_out)) return HIPATTN_OK;
+    if (desc->num_seqs > 0 &&
+        (!k_new || !v_new || !key_cache || !value_cache || !past_lens || !subsequence_begins || !block_indices || !block_indices_begins))
         return fail(HIPATTN_INVALID_ARGUMENT, "rope_append: null pointer");
-    if (desc->cache_dtype == HIPATTN_I8 && (!key_scales || !value_scales))
+    if (desc->num_seqs > 0 && desc->cache_dtype == HIPATTN_I8 && (!key_scales || !value_scales))
         return fail(HIPATTN_INVALID_ARGUMENT, "rope_append: an i8 cache needs key_scales and value_scales");
     const hipattn::KvWriteParams w = make_write_params(desc, k_new, v_new, key_cache, value_cache, past_lens, subsequence_begins,
                                                        block_indices, block_indices_begins);

@@ -63,7 +63,7 @@ struct Slot {
 };
 __device__ __forceinline__ Slot slot_of_token(const RopeAppendParams& p, int t, int lane) {
     Slot r{-1, -1, -1};
-    if (t < p.subsequence_begins[0] || t >= p.subsequence_begins[p.num_seqs]) return r;
+    if (p.num_seqs == 0 || t < p.subsequence_begins[0] || t >= p.subsequence_begins[p.num_seqs]) return r;
     r.sequence = locate_sequence(p.subsequence_begins, p.num_seqs, t, lane);
     r.position = p.past_lens[r.sequence] + (t - p.subsequence_begins[r.sequence]);
     if (r.position < 0) return r;
@@ -544,10 +544,11 @@ bool takes_vector(const RopeAppendParams& p) {
 }  // namespace
 
 hipError_t launch_rope_append(const RopeAppendParams& p, hipStream_t stream) {
-    if (p.num_tokens == 0 || p.num_seqs == 0) return hipSuccess;
-    const bool blocks = p.cache_dtype == HIPATTN_I8;
-    const int64_t block_items = blocks ? (p.num_tokens / p.block_size + 2 * (int64_t)p.num_seqs) * 2 * p.num_heads_kv : 0;
-    const int row_heads = (p.q ? p.num_heads_q : 0) + (blocks ? 0 : 2 * p.num_heads_kv);
+    if (p.num_tokens == 0) return hipSuccess;
+    // (without sequences nothing is stored and no index array looked at: queries alone)
+    const bool stores = p.num_seqs > 0, blocks = p.cache_dtype == HIPATTN_I8;
+    const int64_t block_items = stores && blocks ? (p.num_tokens / p.block_size + 2 * (int64_t)p.num_seqs) * 2 * p.num_heads_kv : 0;
+    const int row_heads = (p.q ? p.num_heads_q : 0) + (stores && !blocks ? 2 * p.num_heads_kv : 0);
     const auto groups_of = [](int64_t waves) { return (waves + kWavesPerGroup - 1) / kWavesPerGroup; };
     if (takes_vector(p)) {
         // a round of rows is what a wavefront has on its way at once

@@ -271,3 +271,23 @@ def test_refusals(hip):
     one = p
     assert L.hipattn_kv_cache_write(ctypes.byref(pa()), one, one, one, one, one, one, one, one, None) == hip.UNSUPPORTED
     assert L.hipattn_paged_attention(ctypes.byref(pa()), one, one, one, one, one, one, one, one, one, one, one, 1 << 30, None) == hip.INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("D,dtype", [(128, BF16), (72, F16), (33, F32)])
+def test_a_batch_without_sequences_copies_its_queries(hip, D, dtype):
+    """Every token is outside every sequence: queries are not turned, nothing is stored, and the index arrays are not looked at."""
+    T, Hq = 5, 6
+    q = W.to_storage(np.random.default_rng(16).standard_normal((T, Hq, D)).astype(np.float32), dtype)[0]
+    up = hip.DeviceBuffer.from_numpy
+    dq, out = up(q), hip.DeviceBuffer(q.nbytes)
+    out.fill(0xFF)
+    table = up(np.ones((8, D), np.float32))
+    rope = hip.RopeAppendDesc(table_dtype=F32, rotary_ndims=D // 2 * 2, table_rows=8, table_row_stride=D)
+    for cache in (I8, F16):
+        pa = hip.PaDesc(dtype, dtype, cache, dtype, Hq, 2, D, 32, 4, T, 0, 8, 0, 0.0, 0, 0)
+        hip.rope_append(pa, rope, dq, None, None, table, table, None, out, *[None] * 8)
+        assert np.array_equal(out.download(q.dtype, q.shape), q)
+        out.fill(0xFF)
+    hip.rope_append(pa, rope, dq, None, None, table, table, None, dq, *[None] * 8)  # in place: as it is
+    assert np.array_equal(dq.download(q.dtype, q.shape), q)
+    hip.rope_append(pa, rope, None, None, None, table, table, None, None, *[None] * 8)
