@@ -225,36 +225,50 @@ __global__ __launch_bounds__(256) void quantize_rows_scalar_kernel(QuantizeParam
     for (int64_t i = threadIdx.x; i < p.width; i += blockDim.x) p.codes[row * p.width + i] = (int8_t)code_of(value(i), inverse);
 }
 
+// `rows_per_group` rows to a workgroup of `lanes`.  A launch of 2^32 threads or more runs modulo 2^32 of them, without an error (a row of
+// three elements to 256 lanes: from 16.8 million rows on): more rows go in several.
+template <typename Kernel>
+void launch_in_runs(Kernel kernel, const QuantizeParams& all, int64_t rows_per_group, int lanes, hipStream_t stream) {
+    const int64_t most = (0xffffffffLL / lanes) * rows_per_group;
+    for (int64_t first = 0; first < all.rows; first += most) {
+        QuantizeParams p = all;
+        p.rows = all.rows - first < most ? all.rows - first : most;
+        p.x = (const uint8_t*)all.x + first * all.x_row_stride * (all.x_dtype == HIPATTN_F32 ? 4 : 2);
+        p.codes += first * all.width;
+        p.scales += first;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((p.rows + rows_per_group - 1) / rows_per_group)), dim3((unsigned)lanes), 0, stream, p);
+    }
+}
+
 template <int kSource>
 void launch(const QuantizeParams& p, bool vector, hipStream_t stream) {
-    const dim3 grid((unsigned)p.rows);
     if (!vector) {
-        hipLaunchKernelGGL(quantize_rows_scalar_kernel<kSource>, grid, dim3(256), 0, stream, p);
+        launch_in_runs(quantize_rows_scalar_kernel<kSource>, p, 1, 256, stream);
         return;
     }
     const int64_t chunks = p.width / 8;
     if (chunks <= 512 && p.rows >= kByWaveRows) {
-        const dim3 groups((unsigned)((p.rows + kRowsPerGroup - 1) / kRowsPerGroup)), lanes(64 * kRowsPerGroup);
+        const auto by_wave = [&](auto kernel) { launch_in_runs(kernel, p, kRowsPerGroup, 64 * kRowsPerGroup, stream); };
         if (chunks <= 64)
-            hipLaunchKernelGGL((quantize_rows_by_wave_kernel<kSource, 1>), groups, lanes, 0, stream, p);
+            by_wave(quantize_rows_by_wave_kernel<kSource, 1>);
         else if (chunks <= 128)
-            hipLaunchKernelGGL((quantize_rows_by_wave_kernel<kSource, 2>), groups, lanes, 0, stream, p);
+            by_wave(quantize_rows_by_wave_kernel<kSource, 2>);
         else if (chunks <= 256)
-            hipLaunchKernelGGL((quantize_rows_by_wave_kernel<kSource, 4>), groups, lanes, 0, stream, p);
+            by_wave(quantize_rows_by_wave_kernel<kSource, 4>);
         else
-            hipLaunchKernelGGL((quantize_rows_by_wave_kernel<kSource, 8>), groups, lanes, 0, stream, p);
+            by_wave(quantize_rows_by_wave_kernel<kSource, 8>);
         return;
     }
     // one chunk a lane up to 512 lanes, then more chunks.  A GLU has more lanes instead of a fourth chunk (8,192 rows of 14,336 144 -> 134
     // us, 128 rows 7.1 -> 5.8)
     const int keep = chunks <= 512 ? 1 : chunks <= (kSource == HIPOPS_QUANTIZE_GLU ? 2048 : 1024) ? 2 : 4;
-    const dim3 block((unsigned)((chunks + 64 * keep - 1) / (64 * keep) * 64));
+    const int lanes = (int)((chunks + 64 * keep - 1) / (64 * keep) * 64);
     if (keep == 1)
-        hipLaunchKernelGGL((quantize_rows_kernel<kSource, 1>), grid, block, 0, stream, p);
+        launch_in_runs(quantize_rows_kernel<kSource, 1>, p, 1, lanes, stream);
     else if (keep == 2)
-        hipLaunchKernelGGL((quantize_rows_kernel<kSource, 2>), grid, block, 0, stream, p);
+        launch_in_runs(quantize_rows_kernel<kSource, 2>, p, 1, lanes, stream);
     else
-        hipLaunchKernelGGL((quantize_rows_kernel<kSource, 4>), grid, block, 0, stream, p);
+        launch_in_runs(quantize_rows_kernel<kSource, 4>, p, 1, lanes, stream);
 }
 
 bool float_dtype(int d) { return d == HIPATTN_F32 || d == HIPATTN_F16 || d == HIPATTN_BF16; }

@@ -328,3 +328,17 @@ def test_rows_of_zeros_without_an_epsilon(hip, ops, rows, width, gamma, dtype): 
     assert not codes[1::2].any() and np.array_equal(scales[1::2], np.zeros(len(scales[1::2]), np.float32))
     e = exact[::2].astype(np.float64)
     near(codes[::2], scales[::2], e / np.sqrt((e ** 2).mean(1, keepdims=True)) * np.asarray(gv, np.float64))
+
+
+def test_more_rows_than_a_launch_takes(hip, ops):  # noqa: F811
+    """A launch has at most 2^32 threads: 16.8 million rows of 256 of them, 67 million of 64."""
+    for rows, width in (((1 << 24) + 5, 3), ((1 << 26) + 9, 8)):
+        x, codes, scales = hip.DeviceBuffer(rows * width * 2), hip.DeviceBuffer(rows * width), hip.DeviceBuffer(rows * 4)
+        x.fill(0x3C)
+        codes.fill(0x11)
+        scales.fill(0xFF)
+        ops.quantize_rows(ops.QuantizeDesc(0, F16, F16, 0, 1, 1e-5, rows, width, 0), x, None, codes, scales)
+        assert np.all(codes.download(np.int8, (rows * width,)) == 127)
+        assert np.all(scales.download(np.float32, (rows,)) == R.scale_of_peak(np.float32(W.f16_bits_to_f32(np.array([0x3C3C], np.uint16))[0])))
+        for b in (x, codes, scales):
+            b.free()
