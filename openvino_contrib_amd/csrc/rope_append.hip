@@ -22,6 +22,8 @@
 // large copy 5.1 to 5.9), 7,300 tokens of new prompts (32 heads on 8 of 64, neighbours turned, fp16 cache of blocks of 16) 21.4 us (87 MB, 4.1 TB/s);
 // the scalar form takes 197 and 168 us for them.  128 single tokens into an i8 cache 8.6 us, one 4.2: a chain of the sequence's place, its
 // block, that block's scale and its rows.
+#include <algorithm>
+
 #include "kv_cache_write.hpp"
 
 namespace hipattn {
@@ -238,9 +240,10 @@ __device__ __forceinline__ bool find_block_item(const RopeAppendParams& p, int64
     return true;
 }
 
-__global__ __launch_bounds__(64 * kWavesPerGroup) void rope_append_scalar_kernel(RopeAppendParams p, int64_t block_items, int row_heads) {
+__global__ __launch_bounds__(64 * kWavesPerGroup) void rope_append_scalar_kernel(RopeAppendParams p, int64_t first_group, int64_t block_items,
+                                                                                  int row_heads) {
     const int lane = threadIdx.x & 63;
-    int64_t w = (int64_t)blockIdx.x * kWavesPerGroup + (threadIdx.x >> 6);
+    int64_t w = (first_group + blockIdx.x) * kWavesPerGroup + (threadIdx.x >> 6);
     if (w >= block_items) {  // a row
         w -= block_items;
         const int t = (int)(w / row_heads), head = (int)(w % row_heads);
@@ -515,10 +518,10 @@ __device__ __forceinline__ void block_vector(const RopeAppendParams& p, const Bl
 
 // Wavefronts [0, block_items): blocks; behind them `shares` for each token, heads_per_wave heads each.
 template <bool kBf16>
-__global__ __launch_bounds__(64 * kWavesPerGroup) void rope_append_kernel(RopeAppendParams p, int64_t block_items, int row_heads, int heads_per_wave,
-                                                                           int shares) {
+__global__ __launch_bounds__(64 * kWavesPerGroup) void rope_append_kernel(RopeAppendParams p, int64_t first_group, int64_t block_items, int row_heads,
+                                                                           int heads_per_wave, int shares) {
     const int lane = threadIdx.x & 63;
-    const int64_t w = (int64_t)blockIdx.x * kWavesPerGroup + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t w = (first_group + blockIdx.x) * kWavesPerGroup + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (w < block_items) {
         BlockItem item;
         if (find_block_item(p, w, lane, item)) block_vector<kBf16>(p, item, lane);
@@ -549,26 +552,24 @@ hipError_t launch_rope_append(const RopeAppendParams& p, hipStream_t stream) {
     const bool stores = p.num_seqs > 0, blocks = p.cache_dtype == HIPATTN_I8;
     const int64_t block_items = stores && blocks ? (p.num_tokens / p.block_size + 2 * (int64_t)p.num_seqs) * 2 * p.num_heads_kv : 0;
     const int row_heads = (p.q ? p.num_heads_q : 0) + (stores && !blocks ? 2 * p.num_heads_kv : 0);
-    const auto groups_of = [](int64_t waves) { return (waves + kWavesPerGroup - 1) / kWavesPerGroup; };
+    // (a launch of 2^32 threads or more would run modulo 2^32 of them, without an error)
+    const auto launch = [&](auto kernel, int64_t waves, auto... last) -> hipError_t {
+        constexpr int kLanes = 64 * kWavesPerGroup;
+        const int64_t groups = (waves + kWavesPerGroup - 1) / kWavesPerGroup, most = 0xffffffffLL / kLanes;
+        for (int64_t first = 0; first < groups; first += most) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(groups - first, most)), dim3(kLanes), 0, stream, p, first, block_items, row_heads, last...);
+            if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+        }
+        return hipSuccess;
+    };
     if (takes_vector(p)) {
         // a round of rows is what a wavefront has on its way at once
         const int round = kAhead * (64 / (p.head_dim / 16));
-        const int shares = (row_heads + round - 1) / round;
-        const int64_t groups = groups_of(block_items + (int64_t)p.num_tokens * shares);
-        if (groups > 0x7fffffff) return hipErrorInvalidValue;
-        if (groups == 0) return hipSuccess;
-        const dim3 grid((unsigned)groups), block(64 * kWavesPerGroup);
-        if (p.kv_dtype == HIPATTN_BF16)
-            hipLaunchKernelGGL(rope_append_kernel<true>, grid, block, 0, stream, p, block_items, row_heads, round, shares > 0 ? shares : 1);
-        else
-            hipLaunchKernelGGL(rope_append_kernel<false>, grid, block, 0, stream, p, block_items, row_heads, round, shares > 0 ? shares : 1);
-        return hipGetLastError();
+        const int shares = std::max((row_heads + round - 1) / round, 1);
+        const int64_t waves = block_items + (row_heads > 0 ? (int64_t)p.num_tokens * shares : 0);
+        return launch(p.kv_dtype == HIPATTN_BF16 ? rope_append_kernel<true> : rope_append_kernel<false>, waves, round, shares);
     }
-    const int64_t groups = groups_of(block_items + (int64_t)p.num_tokens * row_heads);
-    if (groups > 0x7fffffff) return hipErrorInvalidValue;
-    if (groups == 0) return hipSuccess;
-    hipLaunchKernelGGL(rope_append_scalar_kernel, dim3((unsigned)groups), dim3(64 * kWavesPerGroup), 0, stream, p, block_items, row_heads);
-    return hipGetLastError();
+    return launch(rope_append_scalar_kernel, block_items + (int64_t)p.num_tokens * row_heads);
 }
 
 }  // namespace hipattn

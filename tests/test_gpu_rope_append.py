@@ -291,3 +291,22 @@ def test_a_batch_without_sequences_copies_its_queries(hip, D, dtype):
     hip.rope_append(pa, rope, dq, None, None, table, table, None, dq, *[None] * 8)  # in place: as it is
     assert np.array_equal(dq.download(q.dtype, q.shape), q)
     hip.rope_append(pa, rope, None, None, None, table, table, None, None, *[None] * 8)
+
+
+def test_more_rows_than_a_launch_takes(hip):
+    """A launch has at most 2^32 threads, 67 million rows of a wavefront each: tokens of 62 query heads, a key and a value."""
+    T, Hq, bs = (1 << 20) + 300, 62, 1024
+    q, new, out = hip.DeviceBuffer(2 * T * Hq), hip.DeviceBuffer(2 * T), hip.DeviceBuffer(2 * T * Hq)
+    blocks = -(-T // bs)
+    caches = [hip.DeviceBuffer(2 * blocks * bs) for _ in range(2)]
+    q.fill(0x3C)
+    new.fill(0x2A)
+    for b in (out, *caches):
+        b.fill(0xFF)
+    up = hip.DeviceBuffer.from_numpy
+    index = [up(np.array(a, np.int32)) for a in ([0], [0, T], np.arange(blocks), [0, blocks])]
+    pa = hip.PaDesc(F16, F16, F16, F16, Hq, 1, 1, bs, blocks, T, 1, T, 0, 0.0, 0, 0)
+    hip.rope_append(pa, hip.RopeAppendDesc(), q, new, new, None, None, None, out, *caches, None, None, *index)
+    assert np.all(out.download(np.uint16, (T * Hq,)) == 0x3C3C)
+    for c in caches:
+        assert np.all(c.download(np.uint16, (blocks * bs,))[:T] == 0x2A2A)
