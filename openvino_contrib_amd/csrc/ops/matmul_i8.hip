@@ -241,6 +241,22 @@ hipattn_status matmul_i8(const hipops_matmul_i8_desc* d, const int8_t* a, const 
     const MatmulI8Params p{a, b, a_scales, b_scales, bias, residual, c, d->m, d->n, d->k, d->lda ? d->lda : d->k, d->ldb ? d->ldb : d->k,
                            d->ldc ? d->ldc : d->n, d->c_dtype};
     if ((uintptr_t)workspace % 16) return fail(HIPATTN_INVALID_ARGUMENT, "matmul_i8: workspace must be 16-byte aligned");
+    // A launch of 2^32 threads or more would run modulo 2^32 of them, without an error: calls that could come to that go in pieces.  (Without
+    // LDS a column of results takes 32 lanes; in tiles 128 x 128 of them take 512 at most, the smaller tiles those of few rows.)
+    const int64_t most_n = (int64_t)1 << 26, most_m = (((int64_t)1 << 30) - 1) / ((std::min(d->n, most_n) + 127) / 128);
+    if (d->n > most_n || d->m > most_m) {
+        const int64_t size = d->c_dtype == HIPATTN_F32 ? 4 : 2;
+        const auto from = [](auto* base, int64_t bytes) { return base ? (decltype(base))((const uint8_t*)base + bytes) : nullptr; };
+        for (int64_t i = 0; i < d->m; i += most_m)
+            for (int64_t j = 0; j < d->n; j += most_n) {
+                const hipops_matmul_i8_desc piece{d->c_dtype, std::min(d->m - i, most_m), std::min(d->n - j, most_n), d->k, p.lda, p.ldb, p.ldc};
+                const int64_t at = size * (i * p.ldc + j);
+                if (const hipattn_status st = matmul_i8(&piece, from(a, i * p.lda), from(a_scales, 4 * i), from(b, j * p.ldb), from(b_scales, 4 * j), from(bias, size * j),
+                                                        from(residual, at), from(c, at), workspace, workspace_bytes, stream))
+                    return st;
+            }
+        return HIPATTN_OK;
+    }
     // (tiles that load straight to LDS address a row from the tile's first in 32 bits)
     const bool aligned = (((uintptr_t)a | (uintptr_t)b | (uintptr_t)p.lda | (uintptr_t)p.ldb | (uintptr_t)p.k) & 15) == 0 && p.lda <= (1 << 23) && p.ldb <= (1 << 23);
     const I8Plan plan = plan_of(p.m, p.n, p.k, workspace ? workspace_bytes : 0, aligned);

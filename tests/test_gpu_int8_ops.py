@@ -342,3 +342,31 @@ def test_more_rows_than_a_launch_takes(hip, ops):  # noqa: F811
         assert np.all(scales.download(np.float32, (rows,)) == R.scale_of_peak(np.float32(W.f16_bits_to_f32(np.array([0x3C3C], np.uint16))[0])))
         for b in (x, codes, scales):
             b.free()
+
+
+def test_more_columns_than_a_launch_takes(hip, ops):  # noqa: F811
+    """A launch has at most 2^32 threads, which 2^27 or 2^28 columns of few rows reach."""
+    n, k, m = (1 << 28) + 40, 16, 2
+    a, b, c, bias = hip.DeviceBuffer(m * k), hip.DeviceBuffer(n * k), hip.DeviceBuffer(2 * m * n), hip.DeviceBuffer(2 * n)
+    scales = hip.DeviceBuffer(4 * n)
+    a.fill(1)
+    b.fill(2)
+    bias.fill(0x3C)
+    scales.fill(0x3C)
+    c.fill(0xFF)
+    ops.matmul_i8(ops.MatmulI8Desc(F16, m, n, k, 0, 0, 0), a, None, b, scales, bias, None, c)
+    s, plus = np.full(4, 0x3C, np.uint8).view(np.float32)[0], np.float32(W.f16_bits_to_f32(np.array([0x3C3C], np.uint16))[0])
+    want = W.to_storage(np.array([np.float32(32) * s + plus], np.float32), F16)[0][0]
+    assert np.all(c.download(np.uint16, (m * n,)) == want)
+    # and rows: 2^30 of a column each
+    for x in (a, b, c, bias, scales):
+        x.free()
+    m = (1 << 30) + 70
+    a, b, c, bias = hip.DeviceBuffer(m), hip.DeviceBuffer(1), hip.DeviceBuffer(2 * m), hip.DeviceBuffer(2)
+    a.fill(1)
+    b.fill(2)
+    bias.fill(0x3C)
+    c.fill(0xFF)
+    ops.matmul_i8(ops.MatmulI8Desc(F16, m, 1, 1, 0, 0, 0), a, None, b, None, bias, None, c)
+    want = W.to_storage(np.array([2 + plus], np.float32), F16)[0][0]
+    assert np.all(c.download(np.uint16, (m,)) == want)
