@@ -1,14 +1,14 @@
 // New keys and values into a paged cache with the rotary position embedding applied on the way, and the
 // queries rotated beside them: what stands between a decoder layer's q / k / v projection and its attention, in
-// one launch.  HBM-bound byte moving: every row is read once and written once; a table row is read once per
-// wavefront and token and kept in registers over the token's heads.
+// one launch.  HBM-bound byte moving: every row is read once and written once; a table row is read once by each
+// wavefront of a token and kept in registers over its heads (32 of 128 elements: a token of more takes several wavefronts).
 //
 //   rotate-half:  y[i] = x[i] cos[i] - x[i + h] sin[i],  y[i + h] = x[i + h] cos[i + h] + x[i] sin[i + h],  h = rotary / 2
 //   interleaved:  the same on the pairs (2i, 2i + 1) with cos[i], sin[i]
 // fp32, no product fused with the sum: the stored codes are then defined to the bit.
 //
 // Two kinds of work, chosen by wavefront number:
-//  * rows: the heads of one token (queries; with 16-bit, fp32 and u8 caches also its key and value heads);
+//  * rows: heads of one token (queries; with 16-bit, fp32 and u8 caches also its key and value heads);
 //  * blocks (i8 caches): the new rows of one cache block for one kv head of K or V.  The block's scale follows from
 //    all rows that the call puts there, so the wavefront that owns the block-head reads them, finds the largest magnitude,
 //    and only then stores codes; where the scale grew it also scales the codes that were there.  No atomics, no
@@ -345,7 +345,7 @@ struct Lanes {
 
 constexpr int kAhead = 4;  // rows a lane has on their way
 
-// Heads [first, last) of token t.
+// Heads [first, last) of token t, no more than a round of kAhead rows a lane.
 template <bool kBf16>
 __device__ __forceinline__ void rows_vector(const RopeAppendParams& p, int t, int first, int last, int lane) {
     const Lanes l(p.head_dim, lane);
@@ -356,72 +356,67 @@ __device__ __forceinline__ void rows_vector(const RopeAppendParams& p, int t, in
         if (head < Hq + Hkv) return (const uint16_t*)p.k_new + t * p.k_token + (head - Hq) * p.k_head;
         return (const uint16_t*)p.v_new + t * p.v_token + (head - Hq - Hkv) * p.v_head;
     };
+    // (the rows ahead of the chain of loads that finds the token's place)
     Raw raw[kAhead];
-    const auto load = [&](int head0) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < kAhead; i++) {
-            const int head = head0 + i * l.rows + l.row;
-            if (l.active && head < last) {
-                const uint16_t* const src = source(head);
-                const Unit u = head < Hq + Hkv ? turned : plain;
-                raw[i].lo = *(const uint4_t*)(src + u.d0);
-                raw[i].up = *(const uint4_t*)(src + u.d1);
-            }
+    for (int i = 0; i < kAhead; i++) {
+        const int head = first + i * l.rows + l.row;
+        if (l.active && head < last) {
+            const uint16_t* const src = source(head);
+            const Unit u = head < Hq + Hkv ? turned : plain;
+            raw[i].lo = *(const uint4_t*)(src + u.d0);
+            raw[i].up = *(const uint4_t*)(src + u.d1);
         }
-    };
-    load(first);  // (ahead of the chain of loads that finds the token's place)
+    }
     const Slot slot = slot_of_token(p, t, lane);
     const int64_t row = p.rotary && slot.sequence >= 0 ? table_row(p, t, slot.position) : -1;
     Turn turn;
     if (row >= 0 && turned.rotated) load_turn(p, turned, row, turn);
-    for (int head0 = first; head0 < last; head0 += kAhead * l.rows) {
-        if (head0 != first) load(head0);
 #pragma unroll
-        for (int i = 0; i < kAhead; i++) {
-            const int head = head0 + i * l.rows + l.row;
-            // (wavefront-uniform as long as the pieces of a row reduce among themselves: every lane of a row takes the same way)
-            if (!l.active || head >= last) continue;
-            const bool value = head >= Hq + Hkv;
-            const Unit u = value ? plain : turned;
-            float x[16];
-            floats_of<kBf16>(raw[i], x);
-            if (!value && row >= 0 && turned.rotated) turn_unit(p, turn, x);
-            if (head < Hq) {
-                const Raw out = bits_of<kBf16>(x);
-                uint16_t* const dst = (uint16_t*)p.q_out + t * p.out_token + head * p.out_head;
-                *(uint4_t*)(dst + u.d0) = out.lo;
-                *(uint4_t*)(dst + u.d1) = out.up;
-                continue;
+    for (int i = 0; i < kAhead; i++) {
+        const int head = first + i * l.rows + l.row;
+        // (wavefront-uniform as long as the pieces of a row reduce among themselves: every lane of a row takes the same way)
+        if (!l.active || head >= last) continue;
+        const bool value = head >= Hq + Hkv;
+        const Unit u = value ? plain : turned;
+        float x[16];
+        floats_of<kBf16>(raw[i], x);
+        if (!value && row >= 0 && turned.rotated) turn_unit(p, turn, x);
+        if (head < Hq) {
+            const Raw out = bits_of<kBf16>(x);
+            uint16_t* const dst = (uint16_t*)p.q_out + t * p.out_token + head * p.out_head;
+            *(uint4_t*)(dst + u.d0) = out.lo;
+            *(uint4_t*)(dst + u.d1) = out.up;
+            continue;
+        }
+        const int h = head - Hq - (value ? Hkv : 0);
+        uint8_t* const cache = value ? p.value_cache : p.key_cache;
+        const int64_t cache_row = ((int64_t)slot.block * Hkv + h) * p.block_size + slot.position % p.block_size;
+        if (p.cache_dtype == HIPATTN_U8) {
+            float mn = x[0], mx = x[0];
+#pragma unroll
+            for (int e = 1; e < 16; e++) mn = fminf(mn, x[e]), mx = fmaxf(mx, x[e]);
+            for (int d = 1; d < l.units; d <<= 1) {
+                mn = fminf(mn, __shfl_xor(mn, d, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, d, 64));
             }
-            const int h = head - Hq - (value ? Hkv : 0);
-            uint8_t* const cache = value ? p.value_cache : p.key_cache;
-            const int64_t cache_row = ((int64_t)slot.block * Hkv + h) * p.block_size + slot.position % p.block_size;
-            if (p.cache_dtype == HIPATTN_U8) {
-                float mn = x[0], mx = x[0];
+            float scale = (mx - mn) / 255.0f;
+            if (scale == 0.0f) scale = 0.0001f;
+            const float zp = -mn / scale + 0.0f;  // -0 becomes +0
+            const float inv = 1.0f / scale;
+            int q[2][8];
 #pragma unroll
-                for (int e = 1; e < 16; e++) mn = fminf(mn, x[e]), mx = fmaxf(mx, x[e]);
-                for (int d = 1; d < l.units; d <<= 1) {
-                    mn = fminf(mn, __shfl_xor(mn, d, 64));
-                    mx = fmaxf(mx, __shfl_xor(mx, d, 64));
-                }
-                float scale = (mx - mn) / 255.0f;
-                if (scale == 0.0f) scale = 0.0001f;
-                const float zp = -mn / scale + 0.0f;  // -0 becomes +0
-                const float inv = 1.0f / scale;
-                int q[2][8];
-#pragma unroll
-                for (int e = 0; e < 16; e++) q[e >> 3][e & 7] = (int)fminf(fmaxf(rintf(fmaf(x[e], inv, zp)), 0.0f), 255.0f);
-                if (slot.block < 0) continue;
-                uint8_t* const dst = cache + cache_row * (p.head_dim + 8);
-                if (l.unit == 0) *(float2*)dst = make_float2(scale, zp);
-                *(uint2_t*)(dst + 8 + u.d0) = pack_bytes(q[0]);
-                *(uint2_t*)(dst + 8 + u.d1) = pack_bytes(q[1]);
-            } else if (slot.block >= 0) {
-                uint16_t* const dst = (uint16_t*)cache + cache_row * p.head_dim;
-                const Raw out = p.cache_dtype == HIPATTN_BF16 ? bits_of<true>(x) : bits_of<false>(x);
-                *(uint4_t*)(dst + u.d0) = out.lo;
-                *(uint4_t*)(dst + u.d1) = out.up;
-            }
+            for (int e = 0; e < 16; e++) q[e >> 3][e & 7] = (int)fminf(fmaxf(rintf(fmaf(x[e], inv, zp)), 0.0f), 255.0f);
+            if (slot.block < 0) continue;
+            uint8_t* const dst = cache + cache_row * (p.head_dim + 8);
+            if (l.unit == 0) *(float2*)dst = make_float2(scale, zp);
+            *(uint2_t*)(dst + 8 + u.d0) = pack_bytes(q[0]);
+            *(uint2_t*)(dst + 8 + u.d1) = pack_bytes(q[1]);
+        } else if (slot.block >= 0) {
+            uint16_t* const dst = (uint16_t*)cache + cache_row * p.head_dim;
+            const Raw out = p.cache_dtype == HIPATTN_BF16 ? bits_of<true>(x) : bits_of<false>(x);
+            *(uint4_t*)(dst + u.d0) = out.lo;
+            *(uint4_t*)(dst + u.d1) = out.up;
         }
     }
 }
