@@ -1200,7 +1200,7 @@ __device__ __forceinline__ void run_both(const Tile& t0, const Tile& t1, uint8_t
 
 // One workgroup per (128-row query tile of a multi-token sequence, pair of query heads) or, with an
 // odd number of query heads per kv head, per (pair of query tiles, query head).
-template <bool kPad = false>
+template <bool kPad = false, bool kI8 = false>
 __device__ __forceinline__ Tile paged_group_tile(const PagedParams& p, int s, int qt, int h, bool has_work) {
     const int D = kPad ? p.head_dim : kD;
     const int G = p.num_heads_q / p.num_heads_kv;
@@ -1223,7 +1223,7 @@ __device__ __forceinline__ Tile paged_group_tile(const PagedParams& p, int s, in
     t.q_dtype = p.q_dtype;
     t.out_dtype = p.out_dtype;
     t.head_dim = D;
-    const int row_bytes = p.cache_dtype == HIPATTN_U8 ? kU8RowBytes : p.cache_dtype == HIPATTN_I8 ? D : D * 2;
+    const int row_bytes = kI8 ? D : p.cache_dtype == HIPATTN_U8 ? kU8RowBytes : D * 2;
     const int64_t head_off = (int64_t)(h / G) * p.block_size * row_bytes;
     t.k = p.key_cache + head_off;
     t.v = p.value_cache + head_off;
@@ -1233,7 +1233,7 @@ __device__ __forceinline__ Tile paged_group_tile(const PagedParams& p, int s, in
     t.block_stride = (int64_t)p.num_heads_kv * p.block_size * row_bytes;
     t.block_size = p.block_size;
     t.block_shift = __builtin_ctz(p.block_size);
-    if (p.cache_dtype == HIPATTN_I8) {
+    if constexpr (kI8) {
         t.k_scales = p.key_scales + h / G;
         t.v_scales = p.value_scales + h / G;
         t.scale_stride = p.num_heads_kv;
@@ -1285,8 +1285,8 @@ __device__ __forceinline__ void paged_prefill_item(const PagedParams& p, int ind
     // of query heads per kv head, two consecutive query tiles of one head: the item of the even
     // tile does both, the item of the odd tile has nothing left to do.
     if (!pair_heads && (qt & 1)) return;
-    const Tile t0 = paged_group_tile<kPad>(p, s, qt, h0, true);
-    const Tile t1 = pair_heads ? paged_group_tile<kPad>(p, s, qt, h0 + 1, true) : paged_group_tile<kPad>(p, s, qt + 1, h0, qt + 1 < tiles_s);
+    const Tile t0 = paged_group_tile<kPad, kI8>(p, s, qt, h0, true);
+    const Tile t1 = pair_heads ? paged_group_tile<kPad, kI8>(p, s, qt, h0 + 1, true) : paged_group_tile<kPad, kI8>(p, s, qt + 1, h0, qt + 1 < tiles_s);
     if constexpr (kShadow) {
         const int begin = p.subsequence_begins[s], end = p.subsequence_begins[s + 1];
         int64_t block = -1;  // the sequence's first in the copy
