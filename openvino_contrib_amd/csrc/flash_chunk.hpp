@@ -1289,24 +1289,26 @@ __device__ __forceinline__ void paged_prefill_item(const PagedParams& p, int ind
     const Tile t1 = pair_heads ? paged_group_tile<kPad, kI8>(p, s, qt, h0 + 1, true) : paged_group_tile<kPad, kI8>(p, s, qt + 1, h0, qt + 1 < tiles_s);
     if constexpr (kShadow) {
         const int begin = p.subsequence_begins[s], end = p.subsequence_begins[s + 1];
-        int64_t block = -1;  // the sequence's first in the copy
-        int from = 0;        // and which of its own that is
-        if (p.shadow_table != nullptr && end - begin >= kShadowTokens && t0.table_len > 0) {
-            if constexpr (kI8) {
-                block = p.shadow_base[s];
-                from = p.sliding_window > 0 ? (max(0, p.past_lens[s] - p.sliding_window + 1) & ~(kTileK - 1)) / p.block_size : 0;
-            } else if (p.past_lens[s] == 0 && begin >= 0 && end <= p.num_tokens) {
-                block = shadow_block(begin, s, p.block_size);
-            }
+        const bool may_have = p.shadow_table != nullptr && end - begin >= kShadowTokens && t0.table_len > 0;
+        int64_t block;  // the sequence's first in the copy
+        int from = 0;   // and which of its own that is
+        bool copied;
+        if constexpr (kI8) {
+            block = may_have ? p.shadow_base[s] : -1;
+            copied = block >= 0;
+            from = p.sliding_window > 0 ? (max(0, p.past_lens[s] - p.sliding_window + 1) & ~(kTileK - 1)) / p.block_size : 0;
+        } else {
+            block = shadow_block(begin, s, p.block_size);
+            copied = may_have && p.past_lens[s] == 0 && begin >= 0 && end <= p.num_tokens;
         }
-        if (block >= 0) {
+        if (copied) {
             const int64_t stride = (int64_t)p.num_heads_kv * p.block_size * kRowBytes;
             const int64_t off = block * stride + (int64_t)hkv * p.block_size * kRowBytes;
             const auto in_shadow = [&](Tile t) {
                 t.k = (const uint8_t*)p.shadow_k + off;
                 t.v = (const uint8_t*)p.shadow_v + off;
                 t.table = p.shadow_table + block - from;
-                t.num_blocks = min(t.table_len, (p.past_lens[s] + (end - begin) + p.block_size - 1) / p.block_size) - from;
+                t.num_blocks = min(t.table_len, ((kI8 ? p.past_lens[s] : 0) + (end - begin) + p.block_size - 1) / p.block_size) - from;  // (else: no cached tokens)
                 t.block_stride = stride;
                 return t;
             };
