@@ -325,3 +325,12 @@ def test_values_up_to_the_largest_of_16_bits(hip, seqs):
     b.scales[1] *= 4
     got, q, _, path = run(hip, b, out_dtype=F32)
     assert np.isfinite(got).all(), path
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(32, 1), (48, 3), (24, 1)])
+def test_expanded_prompts_of_shared_kv_heads(hip, Hq, Hkv):
+    """More query heads to a kv head than the kernels take at once: the groups share one copy of the prompts' rows."""
+    for seqs in ([(0, 400), (700, 1), (100, 450), (5, 3)], [(0, 700)]):
+        b = R.Batch(21, seqs, Hq, Hkv, 128, 32)
+        check(hip, b, bound_of(True, F16, F32, True), out_dtype=F32)
+        check(hip, b, bound_of(True, F16, F32, True), out_dtype=F32, window=130, small_workspace=True)
