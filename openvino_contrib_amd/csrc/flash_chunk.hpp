@@ -1290,13 +1290,15 @@ __device__ __forceinline__ void paged_prefill_item(const PagedParams& p, int ind
     if constexpr (kShadow) {
         const int begin = p.subsequence_begins[s], end = p.subsequence_begins[s + 1];
         const bool may_have = p.shadow_table != nullptr && end - begin >= kShadowTokens && t0.table_len > 0;
-        int64_t block;  // the sequence's first in the copy
-        int from = 0;   // and which of its own that is
+        int64_t block = -1;  // the sequence's first in the copy
+        int from = 0;        // and which of its own that is
         bool copied;
         if constexpr (kI8) {
-            block = may_have ? p.shadow_base[s] : -1;
+            if (may_have) {
+                block = p.shadow_base[s];
+                from = p.sliding_window > 0 ? (max(0, p.past_lens[s] - p.sliding_window + 1) & ~(kTileK - 1)) / p.block_size : 0;
+            }
             copied = block >= 0;
-            from = p.sliding_window > 0 ? (max(0, p.past_lens[s] - p.sliding_window + 1) & ~(kTileK - 1)) / p.block_size : 0;
         } else {
             block = shadow_block(begin, s, p.block_size);
             copied = may_have && p.past_lens[s] == 0 && begin >= 0 && end <= p.num_tokens;
