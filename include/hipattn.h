@@ -335,7 +335,8 @@ hipattn_status hipattn_rotate_key_cache(const hipattn_pa_desc* desc, void* key_c
  * 16-bit queries with a head_dim that is a multiple of 8 up to 128, on blocks of 16, 32 or a larger power of two, with at most
  * 16 query heads per kv head or a number that divides into groups of 8 to 16, take the split-context decode kernel (not with
  * alibi_slopes) and, at head size 128, the chunk kernel (with neither alibi_slopes nor sinks).  Other 16-bit calls on power-of-two blocks with
- * a head_dim that is a multiple of 8 up to 256 take the query-tile kernel, everything else the shape-generic ones.
+ * a head_dim that is a multiple of 8 up to 256 take the query-tile kernel (a single token then walks its context alone: at head size 256
+ * 64 sequences of 512 to 8,072 tokens take 6.4 ms, from a u8 cache 0.25), everything else the shape-generic ones.
  * Sequences of 384 new tokens or more have the rows that they attend expanded to fp16 once, in the workspace (at most 256 MiB and
  * 1,024 sequences; hipattn_paged_attention_workspace_size asks for that room where max_context_len bounds it, and a smaller
  * workspace leaves it out).  The chunk kernel works on the fp16 numbers nearest to code * scale (keys: times softmax scale and log2(e) as

@@ -12,8 +12,8 @@ namespace {
 // Up to 32 activation rows: the weights, read once, are most of the time.  A workgroup takes 16 kN weight rows and its eight wavefronts an
 // eighth of k each; a lane's loads are the matrix operands as they stand (16 bytes of k of weight row lane % 16, of kM tiles of 16 activation
 // rows alike), kGroup steps multiplied while the next ones are on their way.  Only the eight partial sums meet in LDS.  One row on
-// 4,096 x 4,096 6.0 us alone (2.8 TB/s: launch and one round of loads; in tiles with LDS 10.1), 32 rows 10.1 (11.5), 64 14.2 (13.4): every workgroup
-// reads all activations, 16 bytes of 16 rows at a time.  Twice the weight rows halve that, where n still fills the device: 32 x 6,144 x 2,048
+// 4,096 x 4,096 6.0 us alone (2.8 TB/s: launch and one round of loads; in tiles with LDS 10.1), 32 rows 10.1 (11.5): every workgroup reads
+// all activations, 16 bytes of 16 rows at a time.  Twice the weight rows halve that, where n still fills the device: 32 x 6,144 x 2,048
 // 10.1 -> 8.6 us (in tiles 10.7), 16 x 28,672 x 4,096 38.4 -> 33.0 (25.0).
 constexpr int kFewWaves = 8;
 
@@ -185,6 +185,7 @@ constexpr TileCost kTileCosts[] = {
 // 39.6 / 37.1; 128 x 4,095 x 14,333 38.9 / 34.9; 100 x 2,001 x 1,001 10.4 / 17.8; 8,191 x 6,143 x 4,097 - / 391).
 constexpr TileCost kAnyCosts[] = {{kI8Any32, 32, 128, 512, 5.63f, 1.12f, 0.746f, 0.763f}, {kI8Any128, 128, 128, 1 << 30, 6.8f, 1.84f, 1.21f, 0.556f}};
 constexpr int kParts[] = {1, 2, 3, 4, 6, 8, 12, 16};
+// (the device's 256 compute units: the other constants were fitted on them and hold for no other number)
 constexpr float kUnits = 256.0f, kBytesPerUs = 8.0e6f, kSumBytesPerUs = 3.88e6f, kSecondLaunch = 2.88f;
 
 I8Plan plan_of(int64_t m, int64_t n, int64_t k, size_t workspace_bytes, bool aligned) {

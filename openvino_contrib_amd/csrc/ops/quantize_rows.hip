@@ -4,7 +4,7 @@
 // HBM-bound: x read once, a byte an element written.  A workgroup takes a row and keeps it in registers (eight elements to a
 // chunk, kKeep chunks a lane) over its reductions: the norm's sum of squares, then the largest magnitude; from 1,024 rows on a wavefront takes
 // one by itself where its registers hold it.  bf16 rows, us: 8,192 of 4,096 plain 16.8 (6.0 TB/s), behind a norm 20.1, 1,111 of 14,336 behind a
-// GLU 20.1 (4.0 TB/s: the activation's instructions), 8,192 of them 115 (6.1 TB/s), 64 of 4,096 behind a norm 3.7, one 2.4.
+// GLU 20.1 (4.0 TB/s: the activation's instructions), 8,192 of them 116 (5.1 TB/s), 64 of 4,096 behind a norm 3.8, one 2.5.
 #include "hipops_int8.h"
 #include "ops/ops_common.hpp"
 #include "ops/vec8.hpp"
@@ -259,8 +259,8 @@ void launch(const QuantizeParams& p, bool vector, hipStream_t stream) {
             by_wave(quantize_rows_by_wave_kernel<kSource, 8>);
         return;
     }
-    // one chunk a lane up to 512 lanes, then more chunks.  A GLU has more lanes instead of a fourth chunk (8,192 rows of 14,336 144 -> 134
-    // us, 128 rows 7.1 -> 5.8)
+    // one chunk a lane up to 512 lanes, then more chunks.  A GLU has more lanes instead of a fourth chunk (8,192 rows of 14,336 122 -> 116
+    // us, 128 rows 6.0 -> 5.1)
     const int keep = chunks <= 512 ? 1 : chunks <= (kSource == HIPOPS_QUANTIZE_GLU ? 2048 : 1024) ? 2 : 4;
     const int lanes = (int)((chunks + 64 * keep - 1) / (64 * keep) * 64);
     if (keep == 1)

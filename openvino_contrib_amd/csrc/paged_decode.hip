@@ -109,9 +109,9 @@ __device__ __forceinline__ void plan_block(const PagedParams& p) {
 // kShadowTokens new tokens or more get it, cached tokens included, from the first block that the window leaves; as many as p.shadow_capacity
 // blocks hold, in their order.  Four workgroups to a block, K and V and half the kv heads each; the first one also leaves where each
 // sequence's begin.
-// Measured (us a step, 32 heads on 8, without -> with): six prompts of 100 to 3,000 tokens 189 -> 148, two of 3,000 228 -> 182, one of 1,000
-// 47.5 -> 39.8, eight of 400 55.9 -> 52.7; eight chunks of 512 behind 4,096 tokens (64 heads) 485 -> 389, with a window of that and 120 decode
-// rows 581 -> 513, one of 400 behind 4,096 160 -> 112.
+// Measured (us a step, 32 heads on 8, without -> with): six prompts of 100 to 3,000 tokens 229 -> 189, two of 3,000 210 -> 178, one of 1,000
+// 46.1 -> 39.3, eight of 400 56.5 -> 55.1; eight chunks of 512 behind 4,096 tokens (64 heads) 663 -> 571, with a window of that and 120 decode
+// rows of 1,000 to 6,950 890 -> 689, one of 400 behind 4,096 150 -> 117.
 __device__ __forceinline__ void expand_blocks_i8(const PagedParams& p, int workgroup) {
     const int lane = threadIdx.x & 63, index = workgroup >> 2, part = workgroup & 3;
     const bool leaves = workgroup == 0 && threadIdx.x < 64;

@@ -18,9 +18,9 @@
 // (interleaved, and the part that is not rotated), so that both partners of a pair are in one lane and memory is
 // accessed sixteen bytes at a time.  No counterpart in the reference.
 //
-// Measured: eight chunks of 400 to 512 tokens (64 heads on 8 of 128, bf16, a packed projection, i8 cache of blocks of 32) 34.5 us (154 MB, 4.5 TB/s; a
-// large copy 5.1 to 5.9), 7,300 tokens of new prompts (32 heads on 8 of 64, neighbours turned, fp16 cache of blocks of 16) 21.4 us (87 MB, 4.1 TB/s);
-// the scalar form takes 197 and 168 us for them.  128 single tokens into an i8 cache 8.6 us, one 4.2: a chain of the sequence's place, its
+// Measured: eight chunks of 400 to 512 tokens (64 heads on 8 of 128, bf16, a packed projection, i8 cache of blocks of 32) 34.9 us (154 MB, 4.4 TB/s; a
+// large copy 5.1 to 5.9), 7,300 tokens of new prompts (32 heads on 8 of 64, neighbours turned, fp16 cache of blocks of 16) 21.2 us (87 MB, 4.1 TB/s);
+// the scalar form takes 197 and 168 us for them.  128 single tokens into an i8 cache 8.5 us, one 4.3: a chain of the sequence's place, its
 // block, that block's scale and its rows.
 #include <algorithm>
 
