@@ -58,8 +58,9 @@ hipattn_status hipops_route_experts(const hipops_route_desc* desc, const void* l
  *   r = order[p] / order_divisor, or p where order is NULL (a_rows is at least rows then).
  * a [a_rows, k], rows lda bytes apart, with scales as there (strides both 0: 1 and a_rows); b [experts, n, k] and b_scales
  * [experts, ceil(n / 128), ceil(k / 128)] packed.  begins lies on the device; the call looks at `rows` places at most, and rows of c
- * behind begins[experts] stay as they are.  An entry of begins outside [0, rows] or smaller than the one before it, or one of order that names no
- * row of a, gives undefined results in the places concerned; nothing outside the arrays is read or written.
+ * ahead of begins[0] and behind begins[experts] stay as they are, their scales too.  An entry of begins outside [0, rows] or smaller than
+ * the one before it, or one of order that names no row of a, gives undefined results in the places concerned; nothing outside the arrays is
+ * read or written.
  * c: [rows, n] of F32 / F16 / BF16, packed; where `gated` is set, [rows, n / 2]: the GLU of the halves of that row (glu_activation,
  * glu_gate_first as hipops_glu), in fp32 and rounded once.  c_dtype HIPOPS_F8_E4M3 (gated alone): that GLU as codes [rows, n / 2] with
  * c_scales [ceil(n / 2 / 128), rows], as hipops_quantize_fp8 leaves them: the rows of the next product.  c_scales is not looked at otherwise.

@@ -280,7 +280,7 @@ inline int64_t most_expert_tiles(const MatmulFp8Params& p, int64_t rows) {
     return (places < p.experts ? places : (int64_t)p.experts) + places / rows;
 }
 
-// codes of `rows` rows as quantize_fp8 makes them, rows from *row_limit - row_first on left alone
+// codes of `rows` rows as quantize_fp8 makes them; of an experts' product, those of places between *row_begin and *row_limit alone (row r is place row_first + r)
 struct QuantizeFp8Params {
     const void* x;
     const void* gamma;
@@ -289,7 +289,8 @@ struct QuantizeFp8Params {
     int64_t rows, width, x_row_stride, scale_row, scale_block;
     int x_dtype, gamma_dtype, activation, gate_first;
     float eps;
-    const int32_t* row_limit;  // null, or of the rows of an experts' product: how many are real, counted from row_first on
+    const int32_t* row_begin;  // on the device, with row_limit; both null: all rows
+    const int32_t* row_limit;
     int64_t row_first;
 };
 hipError_t launch_quantize_fp8(int source, const QuantizeFp8Params& p, hipStream_t stream);  // quantize_fp8.hip

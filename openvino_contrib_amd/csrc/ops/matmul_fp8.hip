@@ -251,7 +251,7 @@ hipattn_status matmul_fp8_experts(const hipops_matmul_fp8_experts_desc* d, const
         if (e == hipSuccess && codes) {
             const int64_t width = d->n / 2;
             const QuantizeFp8Params q{workspace, nullptr, (uint8_t*)c + first * width, c_scales + first, p.last_place - first, width, width, 1, d->rows,
-                                      HIPATTN_F32, 0, 0, 0, 0.0f, begins + d->experts, first};
+                                      HIPATTN_F32, 0, 0, 0, 0.0f, begins, begins + d->experts, first};
             e = launch_quantize_fp8(HIPOPS_QUANTIZE_PLAIN, q, stream);
         } else if (!codes) {
             p.c = (uint8_t*)p.c + (d->c_dtype == HIPATTN_F32 ? 4 : 2) * at_once * p.ldc;

@@ -30,7 +30,8 @@ __device__ __forceinline__ float inverse_rms(const QuantizeFp8Params& p, float s
     return square == 0.0f ? 0.0f : 1.0f / sqrtf(square);
 }
 __device__ __forceinline__ bool real_row(const QuantizeFp8Params& p, int64_t row) {
-    return row < p.rows && (p.row_limit == nullptr || p.row_first + row < (int64_t)*p.row_limit);
+    if (row >= p.rows) return false;
+    return p.row_limit == nullptr || (p.row_first + row >= (int64_t)*p.row_begin && p.row_first + row < (int64_t)*p.row_limit);
 }
 // another lane's number, without the way through LDS that a shuffle takes; 0 in rows of lanes that the control leaves out
 template <int kControl, int kRows>
@@ -291,7 +292,7 @@ hipattn_status quantize_fp8(const hipops_quantize_fp8_desc* d, const void* x, co
     if (d->rows == 0) return HIPATTN_OK;
     if (!x || !codes || !scales) return fail(HIPATTN_INVALID_ARGUMENT, "quantize_fp8: null pointer");
     const QuantizeFp8Params p{x, gamma, codes, scales, d->rows, d->width, d->x_row_stride ? d->x_row_stride : taken, row ? row : 1, row ? block : d->rows,
-                              d->x_dtype, d->gamma_dtype, d->glu_activation, d->glu_gate_first, d->eps, nullptr, 0};
+                              d->x_dtype, d->gamma_dtype, d->glu_activation, d->glu_gate_first, d->eps, nullptr, nullptr, 0};
     if (const hipError_t e = launch_quantize_fp8(d->source, p, stream); e != hipSuccess) return fail(HIPATTN_HIP_ERROR, "quantize_fp8: %s", hipGetErrorString(e));
     return HIPATTN_OK;
 }

@@ -356,6 +356,47 @@ def test_some_of_the_experts(hip, ops, which):  # noqa: F811
     off(values(raw[p], BF16), ref[p], size[p], terms[p], k, BF16)
 
 
+@pytest.mark.parametrize("which", ["few", "decode", "uneven", "large"])
+@pytest.mark.parametrize("rows_at_once", [0, 7])
+def test_codes_of_some_of_the_experts(hip, ops, which, rows_at_once):  # noqa: F811
+    """The same for codes, in a workspace for all places and for some at a time: two calls, for the first and the last experts, make one result in either order, and
+    places of neither stay as they are."""
+    import ctypes
+
+    n, k = 512, 512
+    c = experts_case(12, COUNTS[which], n, k, tokens=50, top_k=2)
+    ref, size, _ = experts_reference(c)
+    half, E, spare = n // 2, c["E"], 9
+    rows = c["rows"] + spare
+    if rows_at_once and c["rows"] > 200:
+        rows_at_once = 130
+    up = hip.DeviceBuffer.from_numpy
+    a, sa, begins, order = up(c["a"]), up(np.ascontiguousarray(c["sa"].T)), up(c["begins"]), up(np.concatenate([c["order"], np.full(spare, -5, np.int32)]))
+    cuts = [(E // 4, E // 2), (E // 2, E - 1)]
+    held = {}
+    for turn in (0, 1):
+        out, scales = hip.DeviceBuffer(rows * half), hip.DeviceBuffer(4 * rows * R.blocks(half))
+        out.fill(0x7E)
+        scales.fill(0x7E)
+        for first, last in cuts[::-1] if turn else cuts:
+            d = ops.MatmulFp8ExpertsDesc(E4M3, 1, 0, 1, 2, last - first, rows, n, k, 50)
+            part = type("Part", (), dict(ptr=ctypes.c_void_p(begins.ptr.value + 4 * first), nbytes=begins.nbytes - 4 * first))
+            ws = hip.DeviceBuffer(4 * half * rows_at_once or ops.matmul_fp8_experts_workspace_size(d))
+            ws.fill(0xA5)
+            ops.matmul_fp8_experts(d, a, sa, up(c["b"][first:last]), up(c["sb"][first:last]), part, order, out, scales, ws)
+        held[turn] = out.download(np.uint8, (rows, half)), np.ascontiguousarray(scales.download(np.float32, (R.blocks(half), rows)).T)
+    assert np.array_equal(held[0][0], held[1][0]) and np.array_equal(held[0][1].view(np.uint32), held[1][1].view(np.uint32)), "another result in the other order"
+    raw, s = held[0]
+    p = slice(c["begins"][cuts[0][0]], c["begins"][cuts[1][1]])
+    for outside in (slice(0, p.start), slice(p.stop, rows)):
+        assert np.all(raw[outside] == 0x7E) and np.all(np.ascontiguousarray(s[outside]).view(np.uint8) == 0x7E), "places of other experts were written"
+    each = bounds(k, F32, ref, size, True)
+    gate, pair = slice(0, half), slice(half, n)
+    # (as in check_experts)
+    slack = 1.13 * each[:, gate] * (np.abs(ref[:, pair]) + each[:, pair]) + np.abs(ref[:, gate]) * each[:, pair] + 2.0 ** -20 * np.abs(ref).max(1, keepdims=True) ** 2
+    near(raw[p], s[p], R.gated(ref, 0, 1)[p], slack[p])
+
+
 def test_experts_weights_beyond_32_bits(hip, ops):  # noqa: F811
     """The last of 40 experts lies more than 2^32 bytes behind the first."""
     E, n, k = 40, 8192, 14336
