@@ -182,9 +182,9 @@ hipattn_status matmul_fp8(const hipops_matmul_fp8_desc* d, const uint8_t* a, con
     p.a = a, p.b = b, p.a_scales = a_scales, p.b_scales = b_scales, p.bias = bias, p.residual = residual, p.c = c;
     p.m = d->m, p.n = d->n, p.k = d->k, p.lda = d->lda ? d->lda : d->k, p.ldb = d->ldb ? d->ldb : d->k, p.ldc = d->ldc ? d->ldc : d->n, p.c_dtype = d->c_dtype;
     p.a_scale_row = d->a_scale_row_stride ? d->a_scale_row_stride : 1, p.a_scale_block = d->a_scale_row_stride ? d->a_scale_block_stride : d->m;
-    // A launch of 2^32 threads or more would run modulo 2^32 of them, without an error: calls that could come to that go in pieces.  (Tiles of 32 x 128
-    // results take 256 threads, the larger ones fewer for a result.)
-    const int64_t most_n = (int64_t)1 << 22, most_m = (((int64_t)1 << 35) / std::min(d->n, most_n) + 31) / 32 * 32;
+    // A launch of 2^32 threads or more would run modulo 2^32 of them, without an error: calls that could come to that go in pieces.  Tiles of any number of
+    // rows have 128 columns, of which a single one may be there, and 512 threads for 128 rows at most: 2^28 rows of up to 128 columns are 2^30 threads.
+    const int64_t most_n = (int64_t)1 << 22, most_m = (((int64_t)1 << 35) / std::max<int64_t>(std::min(d->n, most_n), 128) + 31) / 32 * 32;
     const int64_t size = d->c_dtype == HIPATTN_F32 ? 4 : 2;
     const bool exact = d->c_dtype == HIPATTN_F32;
     const auto from = [](const void* base, int64_t bytes) { return base ? (const uint8_t*)base + bytes : nullptr; };

@@ -371,3 +371,29 @@ def test_offsets_beyond_32_bits(hip, ops):  # noqa: F811
     ref, size, _ = R.product(a, sa, b, sb)
     for got in results:
         assert np.all(np.abs(got - ref[:len(got)]) <= bounds(k, F32, ref, size)[:len(got)])
+
+
+@pytest.mark.parametrize("n,k", [(2, 1), (1, 16)])
+def test_more_rows_than_a_launch_takes(hip, ops, n, k):  # noqa: F811
+    """2^30 rows and some, at any address and at multiples of 16 bytes, go in several launches: rows of ones, and some others about the launches' ends."""
+    m = (1 << 30) + 5000
+    a, s, c = hip.DeviceBuffer(m * k), hip.DeviceBuffer(m * 4), hip.DeviceBuffer(m * n * 2)
+    a.fill(0x38)
+    s.fill(0x3F)
+    c.fill(0x7E)
+    scale, one = np.full(4, 0x3F, np.uint8).view(np.float32)[0], np.full((1, k), 0x38, np.uint8)
+    rng = np.random.default_rng(n)
+    rows = [0, 1, 127, (1 << 28) - 1, 1 << 28, (1 << 29) + 77, (1 << 30) - 1, 1 << 30, m - 1]
+    some = R.codes_of_normals(rng, (len(rows), k))
+    b = R.codes_of_normals(rng, (n, k))
+    for r, x in zip(rows, some):
+        hip.check(hip.lib().hipattn_memcpy_h2d_async(ctypes.c_void_p(a.ptr.value + r * k), x.ctypes.data_as(ctypes.c_void_p), k, None))
+    hip.check(hip.lib().hipattn_stream_synchronize(None))
+    ops.matmul_fp8(ops.MatmulFp8Desc(F16, m, n, k), a, s, hip.DeviceBuffer.from_numpy(b), hip.DeviceBuffer.from_numpy(np.full((1, 1), 0.01, np.float32)), None, None, c)
+    got = c.download(np.uint16, (m, n))
+    # a block's sum of 16 products or one: bounds() with the instruction's share, which is not there for one
+    ref, size, _ = R.product(np.concatenate([some, one]), np.full((len(rows) + 1, 1), scale), b, np.full((1, 1), 0.01, np.float32))
+    assert np.all(np.abs(values(got[rows], F16) - ref[:-1]) <= bounds(k, F16, ref, size)[:-1])
+    assert np.all(np.abs(values(got[2], F16) - ref[-1]) <= bounds(k, F16, ref, size)[-1])
+    got[rows] = got[2]
+    assert np.all(got == got[2])
