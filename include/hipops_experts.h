@@ -33,8 +33,9 @@ extern "C" {
  * A NaN choice counts as minus infinity; choices of minus infinity are taken, in the order of their index, where nothing else is left, but never
  * from a group that was not kept.
  * begins [experts + 1], order [tokens * top_k], slots [tokens, top_k]: the lists above, or NULL all three.
- * experts <= 1024, top_k <= 64, groups <= 64 and a divisor of experts.  The workspace holds what
- * hipops_route_experts_workspace_size asks for. */
+ * experts <= 1024, top_k <= 64, groups <= 64 and a divisor of experts; lists of 2^26 tokens at most (their cost grows with the square of the
+ * tokens: of 2^20 they are a third of the call's 2.5 ms, of 2^24 most of 246).  The workspace holds what hipops_route_experts_workspace_size asks
+ * for; without lists it is not looked at. */
 #define HIPOPS_ROUTE_SOFTMAX 0
 #define HIPOPS_ROUTE_SIGMOID 1
 typedef struct hipops_route_desc {

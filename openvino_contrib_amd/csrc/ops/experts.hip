@@ -453,7 +453,9 @@ hipattn_status checked(const hipops_route_desc* d) {
 // A few tokens are spread out, four to a workgroup: 64 of 256 experts 12.1 us, 15.7 in a run of 16.  From 4,096 on compute units take whole
 // rounds of workgroups, of which each holds one (sixteen wavefronts of 101 registers): as few rounds as leave a run at 128 tokens.  us in runs of 16, 32, 64,
 // 128 and 224 tokens: 8,192 tokens 38.6, 30.0, 44.0, -, -; 16,384 87.6, 54.3, 47.2, -, -; 60,000 584, -, 183, 155, 246.  Every workgroup of the lists adds up the
-// counts of all runs, so very many tokens go in the longest runs.
+// counts of all runs, so very many tokens go in the longest runs.  That grows with the square of the tokens all the same: the lists of 2^20 tokens of 256 experts
+// 0.8 ms of 2.5, of 2^24 221 of 246, of 2^26 tokens of 8 experts 2,360 of 2,390.  More than 2^26 get no lists.
+static constexpr int64_t kMostListTokens = (int64_t)1 << 26;
 static int run_of(int64_t tokens) {
     if (tokens <= 8) return (int)std::max<int64_t>(tokens, 1);
     if (tokens <= 1024) return 4;
@@ -479,6 +481,7 @@ hipattn_status route_experts(const hipops_route_desc* d, const void* logits, con
     const bool lists = begins || order || slots;
     if (lists && (!begins || (d->tokens > 0 && (!order || !slots)))) return fail(HIPATTN_INVALID_ARGUMENT, "route_experts: begins, order and slots come together");
     if (d->tokens > 0 && (!logits || !indices || !weights)) return fail(HIPATTN_INVALID_ARGUMENT, "route_experts: null pointer");
+    if (lists && d->tokens > kMostListTokens) return fail(HIPATTN_UNSUPPORTED, "route_experts: lists of %lld tokens, more than 2^26", (long long)d->tokens);
     if (d->tokens == 0 && !lists) return HIPATTN_OK;
     RouteParams p{logits, bias, indices, weights, begins, order, slots, nullptr, d->tokens, d->logits_row_stride ? d->logits_row_stride : d->experts, run_of(d->tokens),
                   count_stride_of(d->experts), d->logits_dtype, d->score, d->renormalise, d->experts, d->top_k, std::max(d->groups, 1), d->kept_groups, d->group_top, d->scale};
@@ -490,18 +493,28 @@ hipattn_status route_experts(const hipops_route_desc* d, const void* logits, con
         if ((uintptr_t)workspace % 16) return fail(HIPATTN_INVALID_ARGUMENT, "route_experts: workspace must be 16-byte aligned");
         p.counts = (uint8_t*)workspace;
     }
-    const dim3 grid((unsigned)runs), block((unsigned)(64 * std::min(p.run, kRouteWaves)));
-    if (d->experts <= 64)
-        hipLaunchKernelGGL(route_kernel<1>, grid, block, 0, stream, p);
-    else if (d->experts <= 128)
-        hipLaunchKernelGGL(route_kernel<2>, grid, block, 0, stream, p);
-    else if (d->experts <= 256)
-        hipLaunchKernelGGL(route_kernel<4>, grid, block, 0, stream, p);
-    else if (d->experts <= 512)
-        hipLaunchKernelGGL(route_kernel<8>, grid, block, 0, stream, p);
-    else
-        hipLaunchKernelGGL(route_kernel<16>, grid, block, 0, stream, p);
-    if (lists && runs > 1) hipLaunchKernelGGL(expert_lists_kernel, grid, dim3(kListThreads), 0, stream, p);
+    // (a launch of 2^32 threads or more would run modulo 2^32 of them, without an error: so many tokens, which get no lists, go in several)
+    const unsigned lanes = 64 * std::min(p.run, kRouteWaves);
+    const int64_t most = std::min<int64_t>(runs, 0xffffffffu / lanes);
+    for (int64_t first = 0; first < runs; first += most) {
+        const int64_t token = first * p.run, here = std::min(runs - first, most);
+        RouteParams q = p;
+        q.logits = (const uint8_t*)logits + token * p.row_stride * (d->logits_dtype == HIPATTN_F32 ? 4 : 2);
+        q.indices += token * d->top_k, q.weights += token * d->top_k, q.tokens = std::min(d->tokens - token, here * p.run);
+        const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)here), dim3(lanes), 0, stream, q); };
+        if (d->experts <= 64)
+            launch(route_kernel<1>);
+        else if (d->experts <= 128)
+            launch(route_kernel<2>);
+        else if (d->experts <= 256)
+            launch(route_kernel<4>);
+        else if (d->experts <= 512)
+            launch(route_kernel<8>);
+        else
+            launch(route_kernel<16>);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return fail(HIPATTN_HIP_ERROR, "route_experts: %s", hipGetErrorString(e));
+    }
+    if (lists && runs > 1) hipLaunchKernelGGL(expert_lists_kernel, dim3((unsigned)runs), dim3(kListThreads), 0, stream, p);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return fail(HIPATTN_HIP_ERROR, "route_experts: %s", hipGetErrorString(e));
     return HIPATTN_OK;
 }

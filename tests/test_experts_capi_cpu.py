@@ -159,6 +159,12 @@ def test_route_workspace_refusals():
     refused("hipops_route_experts", d, (P,) * 7 + (None, 0, None), "workspace", capi.WORKSPACE_TOO_SMALL)
 
 
+def test_route_lists_of_too_many_tokens_are_refused():
+    for tokens in ((1 << 26) + 1, 939524097, (1 << 31) - 1):
+        d = ops_capi.RouteDesc(logits_dtype=capi.F16, experts=2, top_k=1, scale=1.0, tokens=tokens)
+        refused("hipops_route_experts", d, (P,) * 8 + (1 << 40, None), "2^26", capi.UNSUPPORTED)
+
+
 def test_combine_refusals():
     def call(word, status=capi.INVALID_ARGUMENT, args=(P,) * 5 + (None,), **fields):
         d = ops_capi.CombineDesc(y_dtype=capi.BF16, out_dtype=capi.BF16, top_k=2, tokens=4, rows=8, n=64)

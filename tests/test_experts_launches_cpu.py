@@ -15,6 +15,11 @@ def product(m, n, k, c_dtype=BF16, offset=0, workspace=0):
     return ("hipops_matmul_fp8", "MatmulFp8Desc", dict(c_dtype=c_dtype, m=m, n=n, k=k), [P + offset, P, P, P, None, None, P, P if workspace else None, workspace, None])
 
 
+def routing(tokens, experts, top_k, lists):
+    return ("hipops_route_experts", "RouteDesc", dict(logits_dtype=F16, renormalise=1, experts=experts, top_k=top_k, scale=1.0, tokens=tokens),
+            [P, None, P, P] + [P if lists else None] * 3 + [P, 1 << 50, None])
+
+
 def fits(launch):
     return 0 < launch.threads < 1 << 32 and launch.grid[1] <= 65535 and launch.grid[2] <= 65535
 
@@ -42,3 +47,19 @@ def test_products_of_any_size():
     for call, (status, error, found) in zip(calls, launches(*calls)):
         assert status == 0, error
         assert found and all(fits(l) for l in found), (call, [l for l in found if not fits(l)])
+
+
+@pytest.mark.parametrize("tokens", [939524096, (1 << 30) + 1, (1 << 31) - 1])
+def test_routing_of_very_many_tokens(tokens):
+    for status, error, found in launches(*[routing(tokens, experts, 1, False) for experts in (1, 128, 256, 512, 1024)]):
+        assert status == 0, error
+        assert len(found) > 1 and all(fits(l) for l in found), found
+        assert sum(l.grid[0] for l in found) == -(-tokens // 224)
+
+
+def test_routing_of_any_size():
+    rng = random.Random(2)
+    calls = [routing(sizes(rng, 1 << 26), rng.choice((1, 8, 60, 128, 1024)), 1, lists) for lists in (True, False) for _ in range(100)]
+    for call, (status, error, found) in zip(calls, launches(*calls)):
+        assert status == 0, error
+        assert found and all(fits(l) for l in found), (call, found)

@@ -134,6 +134,32 @@ def test_lists_of_one_sought_expert(hip, ops):  # noqa: F811
     check_routing(hip, ops, -logits, None, 1, score="sigmoid")
 
 
+def test_routing_of_more_tokens_than_a_launch_takes(hip, ops):  # noqa: F811
+    """224 tokens to a workgroup of 1,024 threads: 2^32 of those are passed, and the call (without lists) goes in two launches.  Rows of equal logits, some others
+    about the launches' ends."""
+    import ctypes
+
+    most = 224 * ((1 << 32) // 1024 - 1)
+    tokens = most + 5000
+    logits, indices, weights = hip.DeviceBuffer(4 * tokens), hip.DeviceBuffer(4 * tokens), hip.DeviceBuffer(4 * tokens)
+    logits.fill(0)
+    indices.fill(0xEE)
+    weights.fill(0xEE)
+    rows, row = [3, 1 << 28, most - 1, most, most + 300, tokens - 1], np.array([-1, 1], np.float16)
+    for r in rows:
+        hip.check(hip.lib().hipattn_memcpy_h2d_async(ctypes.c_void_p(logits.ptr.value + 4 * r), row.ctypes.data_as(ctypes.c_void_p), 4, None))
+    hip.check(hip.lib().hipattn_stream_synchronize(None))
+    ops.route_experts(ops.RouteDesc(logits_dtype=F16, experts=2, top_k=1, scale=3.0, tokens=tokens), logits, None, indices, weights)
+    got = indices.download(np.int32, (tokens,))
+    assert np.all(got[rows] == 1)
+    got[rows] = 0
+    assert not got.any()
+    got = weights.download(np.float32, (tokens,))
+    assert np.all(np.abs(got[rows] - 3 / (1 + np.exp(-2.0))) <= 3 * 2.0 ** -23)
+    got[rows] = 1.5
+    assert np.all(got == 1.5)
+
+
 # ------------------------------------------------------------------------------ products
 def experts_case(seed, counts, n, k, tokens=None, top_k=1):
     """Codes and lists of experts with `counts` rows; tokens: of that many rows of a, each place a random one."""
