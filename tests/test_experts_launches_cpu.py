@@ -20,6 +20,19 @@ def routing(tokens, experts, top_k, lists):
             [P, None, P, P] + [P if lists else None] * 3 + [P, 1 << 50, None])
 
 
+def experts_product(experts, rows, n, k, c_dtype, gated=0, workspace=1 << 30):
+    return ("hipops_matmul_fp8_experts", "MatmulFp8ExpertsDesc", dict(c_dtype=c_dtype, gated=gated, order_divisor=1, experts=experts, rows=rows, n=n, k=k, a_rows=50),
+            [P, P, P, P, P, P, P, P, P, workspace, None])
+
+
+def quantising(rows, width, source=0):
+    return ("hipops_quantize_fp8", "QuantizeFp8Desc", dict(source=source, x_dtype=F16, gamma_dtype=F16, rows=rows, width=width), [P, None, P, P, None])
+
+
+def combining(tokens, n, y_dtype):
+    return ("hipops_combine_experts", "CombineDesc", dict(y_dtype=y_dtype, out_dtype=F16, top_k=2, tokens=tokens, rows=5, n=n), [P] * 5 + [None])
+
+
 def fits(launch):
     return 0 < launch.threads < 1 << 32 and launch.grid[1] <= 65535 and launch.grid[2] <= 65535
 
@@ -63,3 +76,32 @@ def test_routing_of_any_size():
     for call, (status, error, found) in zip(calls, launches(*calls)):
         assert status == 0, error
         assert found and all(fits(l) for l in found), (call, found)
+
+
+def test_the_other_calls_of_any_size():
+    rng, calls = random.Random(3), []
+    while len(calls) < 800:
+        rows, n = sizes(rng, (1 << 31) - 1), sizes(rng, 1 << 26)
+        if rows * n > 1 << 37:
+            continue
+        gated, experts, k = rng.choice((0, 1)), sizes(rng, 1024), sizes(rng, 65536)
+        c_dtype = rng.choice((F32, F16, BF16, ops_capi.F8_E4M3) if gated else (F32, F16, BF16))
+        calls += [experts_product(experts, rows, max(2, n // 2 * 2), k, c_dtype, gated, rng.choice((1 << 30, 1 << 36))), quantising(rows, n, rng.choice((0, 1, 2))),
+                  combining(rows, n, rng.choice((F32, F16)))]
+    for call, (status, error, found) in zip(calls, launches(*calls)):
+        assert status == 0, error
+        assert found and all(fits(l) for l in found), (call, [l for l in found if not fits(l)][:3])
+
+
+def test_sizes_of_gpu_tests_reach_their_kernels():
+    deep, tiles, by_row, quantise = "matmul_fp8_deep_kernel<", "matmul_fp8_tiles_kernel<", "quantize_fp8_norm_kernel<", "quantize_fp8_kernel<"
+    E4M3 = ops_capi.F8_E4M3
+    rows = (1 << 19) + 3001
+    cases = [(product(2001, 6245, 2048, c_dtype), [deep, tiles]) for c_dtype in (BF16, F16)]
+    cases += [(quantising((1 << 26) + 5000, 3, source), [by_row if source == 1 else quantise] * 2) for source in (0, 1, 2)]
+    cases += [(experts_product(4, 2056, n, k, E4M3, 1, 700 * n // 2 * 4), [deep, quantise] * 3) for n, k in ((512, 1024), (256, 640))]
+    cases += [(experts_product(6, 3086, n, k, E4M3, 1, 700 * n // 2 * 4), [deep, quantise] * 5) for n, k in ((512, 1024), (256, 640))]
+    cases += [(experts_product(4, rows, *how), [kernel] * 2) for how, kernel in (((256, 512, BF16, 0), deep), ((512, 640, F16, 1), deep), ((256, 512, F32, 0), tiles), ((130, 100, BF16, 0), tiles))]
+    for (call, kernels), (status, error, found) in zip(cases, launches(*[call for call, _ in cases])):
+        assert status == 0, error
+        assert len(found) == len(kernels) and all(k in l.kernel for k, l in zip(kernels, found)), (call, found)

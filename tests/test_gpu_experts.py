@@ -315,6 +315,44 @@ def test_experts_codes_in_a_small_workspace(hip, ops):  # noqa: F811
         assert np.array_equal(raw, again) and np.array_equal(scales, again_scales)
 
 
+@pytest.mark.parametrize("which", ["many", "large"])
+@pytest.mark.parametrize("n,k", [(512, 1024), (256, 640)])
+def test_experts_codes_some_rows_at_a_time(hip, ops, which, n, k):  # noqa: F811
+    """The same where some rows at a time are enough for tiles of 256: launches that begin at other places than the first, inside an expert's."""
+    c = experts_case(2, COUNTS[which], n, k, tokens=40)
+    raw, scales = run_experts(hip, ops, c, E4M3)
+    again, again_scales = run_experts(hip, ops, c, E4M3, workspace=700 * n // 2 * 4, spare=5)
+    assert np.array_equal(raw, again) and np.array_equal(scales, again_scales)
+
+
+@pytest.mark.parametrize("n,k,c_dtype,gated", [(256, 512, BF16, 0), (512, 640, F16, 1), (256, 512, F32, 0), (130, 100, BF16, 0)])
+def test_more_places_than_a_launch_takes(hip, ops, n, k, c_dtype, gated):  # noqa: F811
+    """More than 2^19 places go in two launches, which meet inside an expert's: places of the same expert and row have the same bits, and those are right."""
+    begins = np.array([0, 100001, 100001, 520000, (1 << 19) + 3001], np.int32)
+    c = experts_case(n + k, list(np.diff(begins)), n, k, tokens=37, top_k=2)
+    out, width = c["rows"], n // 2 if gated else n
+    up = hip.DeviceBuffer.from_numpy
+    result = hip.DeviceBuffer((out + 3) * width * hip.DTYPE_BYTES[c_dtype])
+    result.fill(0x7E)
+    ops.matmul_fp8_experts(ops.MatmulFp8ExpertsDesc(c_dtype, gated, 0, 1, 2, c["E"], out, n, k, 37), up(c["a"]), up(np.ascontiguousarray(c["sa"].T)), up(c["b"]), up(c["sb"]),
+                           up(begins), up(c["order"]), result)
+    raw = result.download(W.np_storage_dtype(c_dtype), (out + 3, width))
+    assert np.all(raw[out:].view(np.uint8) == 0x7E)
+    expert, row = np.repeat(np.arange(c["E"]), np.diff(begins)), c["order"] // 2
+    _, first, which = np.unique(expert * 37 + row, return_index=True, return_inverse=True)
+    assert np.array_equal(raw[:out], raw[first][which])
+    got = values(raw[first], c_dtype)
+    ref, size, terms = (np.concatenate(x) for x in zip(*[R.product(c["a"][r][None], c["sa"][r][None], c["b"][e], c["sb"][e]) for e, r in zip(expert[first], row[first])]))
+    if not gated:
+        off(got, ref, size, terms, k, c_dtype)
+        return
+    each, gate, pair = bounds(k, F32, ref, size, True), slice(0, width), slice(width, n)
+    # (as in check_experts)
+    slack = 1.13 * each[:, gate] * (np.abs(ref[:, pair]) + each[:, pair]) + np.abs(ref[:, gate]) * each[:, pair] + 2.0 ** -20 * np.abs(ref).max(1, keepdims=True) ** 2
+    y = R.gated(ref, 0, 1)
+    assert np.all(np.abs(got - y) <= slack + HALF_ULP[c_dtype] * np.abs(y) * 1.001 + 3e-8)
+
+
 def test_many_experts(hip, ops):  # noqa: F811
     rng = np.random.default_rng(0)
     for E in (65, 300, 1024):
@@ -500,3 +538,23 @@ def test_combine_rows_beyond_32_bits(hip, ops):  # noqa: F811
     out = hip.DeviceBuffer(n * 4)
     ops.combine_experts(ops.CombineDesc(BF16, F32, 2, 1, rows, n), y, up(np.array([[2.0, 3.0]], np.float32)), up(np.array([[rows - 1, 5]], np.int32)), None, out)
     assert np.all(out.download(np.float32, (n,)) == 5.0)
+
+
+def test_combine_of_more_tokens_than_a_launch_takes(hip, ops):  # noqa: F811
+    """A lane for each of seven columns: 2^32 threads are passed, and the call goes in two launches.  Thirteen rows over and over, added to what is there."""
+    n, rows = 7, 13
+    tokens = 0xFFFFFF00 // n + 3000
+    rng = np.random.default_rng(10)
+    stored, y = W.to_storage(rng.standard_normal((rows, n)), F16)
+    up = hip.DeviceBuffer.from_numpy
+    slots, weights, out = up(np.tile(np.arange(rows, dtype=np.int32), -(-tokens // rows))[:tokens]), hip.DeviceBuffer(4 * tokens), hip.DeviceBuffer(2 * n * tokens)
+    weights.fill(0x3F)
+    out.fill(0x3C)
+    ops.combine_experts(ops.CombineDesc(F16, F16, 1, tokens, rows, n), up(stored), weights, slots, out, out)
+    got = out.download(np.uint16, (tokens, n))
+    weight, residual = (np.full(4, b, np.uint8).view(t)[0].astype(np.float64) for b, t in ((0x3F, np.float32), (0x3C, np.float16)))
+    want = residual + weight * y
+    # one product and one sum in fp32, one rounding
+    assert np.all(np.abs(values(got[:rows], F16) - want) <= 2.0 ** -23 * (residual + np.abs(weight * y)) + HALF_ULP[F16] * np.abs(want) * 1.001 + 3e-8)
+    whole = tokens // rows * rows
+    assert np.all(got[:whole].reshape(-1, rows, n) == got[:rows]) and np.all(got[whole:] == got[:tokens - whole])

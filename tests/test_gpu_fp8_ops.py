@@ -164,6 +164,26 @@ def test_more_rows_than_a_launch_has_threads(hip, ops):  # noqa: F811
     assert np.all(codes.download(np.uint8, (rows, 3)) == want) and np.all(scales.download(np.float32, (rows,)) == s[0, 0])
 
 
+@pytest.mark.parametrize("source", [0, 1, 2])
+@pytest.mark.parametrize("by_row", [False, True])
+def test_more_rows_than_a_quantising_launch_takes(hip, ops, source, by_row):  # noqa: F811
+    """64 lanes a row: 2^26 rows and some go in two launches.  Eleven rows over and over, which the launches' ends do not divide by, are those rows every time."""
+    rows, width = (1 << 26) + 5000, 3
+    some = np.random.default_rng(source).standard_normal((11, width * (2 if source == 2 else 1))).astype(np.float32)
+    want, want_scales, exact, _ = quantised(hip, ops, some, F16, source)
+    if source == 0:
+        ref, ref_scales = R.quantised(exact)
+        assert np.array_equal(R.VALUES[want], R.VALUES[ref]) and np.array_equal(want_scales, ref_scales)
+    x = hip.DeviceBuffer.from_numpy(np.tile(W.to_storage(some, F16)[0], (-(-rows // 11), 1))[:rows])
+    codes, scales = hip.DeviceBuffer(rows * width), hip.DeviceBuffer(rows * 4)
+    codes.fill(0x7F)
+    scales.fill(0xFF)
+    ops.quantize_fp8(ops.QuantizeFp8Desc(source, F16, F16, 0, 1, 1e-5, rows, width, 0, int(by_row), int(by_row)), x, None, codes, scales)
+    for got, pattern in ((codes.download(np.uint8, (rows, width)), want), (scales.download(np.uint32, (rows, 1)), np.ascontiguousarray(want_scales).view(np.uint32))):
+        whole = rows // 11 * 11
+        assert np.all(got[:whole].reshape(-1, 11, pattern.shape[1]) == pattern) and np.all(got[whole:] == pattern[:rows - whole])
+
+
 # ------------------------------------------------------------------------------ products
 def bounds(k, dtype, ref, size, coarse=None):
     """The largest error of each element; coarse: summed by the instruction for 8-bit operands."""
@@ -255,6 +275,12 @@ def test_columns_beside_whole_runs(hip, ops, m, n, k):  # noqa: F811
     """Tiles of 256 rows for whole runs of 64 columns, a launch of its own for the rest, which begins at a block of scales or inside one."""
     product(hip, ops, m, n, k, BF16, bias=True, residual=True)
     product(hip, ops, m, n, k, F16, residual=True, by_row=True, pad=(16, 64, 8), in_place=True)
+
+
+def test_columns_beside_an_odd_number_of_runs(hip, ops):  # noqa: F811
+    """The second launch begins 64 columns into a block of the weights' scales: column 6,208."""
+    product(hip, ops, 2001, 6245, 2048, BF16, bias=True, residual=True)
+    product(hip, ops, 2001, 6245, 2048, F16, residual=True, by_row=True, pad=(16, 64, 8), in_place=True)
 
 
 def far_apart(hip, scales, row, block):
