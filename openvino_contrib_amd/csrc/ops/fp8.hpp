@@ -8,9 +8,7 @@
 
 namespace hipops {
 
-typedef int int4_t __attribute__((ext_vector_type(4)));
 typedef int int8v_t __attribute__((ext_vector_type(8)));
-typedef float float16v_t __attribute__((ext_vector_type(16)));
 
 constexpr int kFp8Block = HIPOPS_FP8_BLOCK;
 constexpr float kFp8Largest = 448.0f;
@@ -58,11 +56,6 @@ __device__ __forceinline__ float4_t mma_fp8_16_exact(int8v_t a, int8v_t b, float
         c = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(a), halves(b), c, 0, 0, 0);
     }
     return c;
-}
-// 32 rows of each operand, 64 bytes of k: lane l holds 32 bytes of row l % 32; register r of the result is row 8 (r / 4) + 4 (l / 32) + r % 4 of a
-// and row l % 32 of b
-__device__ __forceinline__ float16v_t mma_fp8_32(int8v_t a, int8v_t b, float16v_t c) {
-    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
 }
 __device__ __forceinline__ int8v_t joined(uint4_t lo, uint4_t hi) {
     return (int8v_t){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
@@ -273,7 +266,7 @@ hipError_t launch_matmul_fp8_few(const MatmulFp8Params& p, bool exact, hipStream
 template <bool kExperts>
 hipError_t launch_matmul_fp8_deep(const MatmulFp8Params& p, hipStream_t stream);  // matmul_fp8_deep.hip
 template <bool kExperts>
-hipError_t launch_matmul_fp8_tiles(const MatmulFp8Params& p, const Fp8Plan& plan, bool exact, void* workspace, hipStream_t stream);  // matmul_fp8_tiles.hip
+hipError_t launch_matmul_fp8_tiles(const MatmulFp8Params& p, const Fp8Plan& plan, bool exact, void* workspace, hipStream_t stream);  // matmul_fp8_tiles.hpp
 // tiles of `rows` rows that the places of an experts' product can come to
 inline int64_t most_expert_tiles(const MatmulFp8Params& p, int64_t rows) {
     const int64_t places = p.last_place - p.first_place;
