@@ -104,20 +104,12 @@ __device__ __forceinline__ void store8_as(Global to, const float* y) {
 }
 template <int kOut>
 __device__ __forceinline__ void load8_as(Global from, float* y) {
-    if constexpr (kOut == HIPATTN_F32) {
+    static_assert(kOut != HIPATTN_F32, "bias and residual: of dense products alone, which have 16 bits here");
+    const uint4_t w = *(GlobalLoose)from;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const uint4_t w = *(GlobalLoose)(from + 16 * h);
-#pragma unroll
-            for (int e = 0; e < 4; e++) y[4 * h + e] = __uint_as_float(w[e]);
-        }
-    } else {
-        const uint4_t w = *(GlobalLoose)from;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const uint16_t v = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-            y[e] = kOut == HIPATTN_F16 ? f16_bits_to_float(v) : bf16_bits_to_float(v);
-        }
+    for (int e = 0; e < 8; e++) {
+        const uint16_t v = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+        y[e] = kOut == HIPATTN_F16 ? f16_bits_to_float(v) : bf16_bits_to_float(v);
     }
 }
 
@@ -389,9 +381,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 float bias[16];
 #pragma unroll
                 for (int e = 0; e < 16; e++) bias[e] = 0.0f;
-                if (!kExperts && p.bias != nullptr) {
-                    load8_as<kOut>((Global)p.bias + kSize * column, bias);
-                    load8_as<kOut>((Global)p.bias + kSize * (column + 32), bias + 8);
+                if constexpr (!kExperts) {
+                    if (p.bias != nullptr) {
+                        load8_as<kOut>((Global)p.bias + kSize * column, bias);
+                        load8_as<kOut>((Global)p.bias + kSize * (column + 32), bias + 8);
+                    }
                 }
                 Global other = kExperts || p.residual == nullptr ? nullptr : (Global)p.residual + kSize * first;
 #pragma unroll
@@ -399,13 +393,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                     if (16 * i < rows) {
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            float y[8], r[8];
+                            float y[8];
 #pragma unroll
                             for (int e = 0; e < 8; e++) y[e] = acc[2 * h + (e >> 2)][i][e & 3] + bias[8 * h + e];
-                            if (other != nullptr) {
-                                load8_as<kOut>(other + 32 * kSize * h, r);
+                            if constexpr (!kExperts) {
+                                if (other != nullptr) {
+                                    float r[8];
+                                    load8_as<kOut>(other + 32 * kSize * h, r);
 #pragma unroll
-                                for (int e = 0; e < 8; e++) y[e] += r[e];
+                                    for (int e = 0; e < 8; e++) y[e] += r[e];
+                                }
                             }
                             store8_as<kOut>(to + 32 * kSize * h, y);
                         }
@@ -443,12 +440,14 @@ hipError_t launch_matmul_fp8_deep(const MatmulFp8Params& p, hipStream_t stream) 
     g.tiles_n = (int)(((p.gated ? p.n / 2 : p.n) + columns - 1) / columns);
     const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n, grid = 8 * ((tiles < 256 ? tiles + 7 : 256) / 8);
     const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(512), 0, stream, Arguments{p, g}); };
-    if (p.c_dtype == HIPATTN_F32)
-        launch(matmul_fp8_deep_kernel<kExperts, HIPATTN_F32>);
-    else if (p.c_dtype == HIPATTN_F16)
+    if (p.c_dtype == HIPATTN_F16) {
         launch(matmul_fp8_deep_kernel<kExperts, HIPATTN_F16>);
-    else
+    } else if (p.c_dtype == HIPATTN_BF16) {
         launch(matmul_fp8_deep_kernel<kExperts, HIPATTN_BF16>);
+    } else {  // (of experts: what becomes codes.  Results in fp32 are exact products, which these tiles do not have)
+        if constexpr (!kExperts) return hipErrorInvalidValue;
+        if constexpr (kExperts) launch(matmul_fp8_deep_kernel<true, HIPATTN_F32>);
+    }
     return hipGetLastError();
 }
 template hipError_t launch_matmul_fp8_deep<false>(const MatmulFp8Params&, hipStream_t);

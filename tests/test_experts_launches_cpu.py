@@ -105,3 +105,13 @@ def test_sizes_of_gpu_tests_reach_their_kernels():
     for (call, kernels), (status, error, found) in zip(cases, launches(*[call for call, _ in cases])):
         assert status == 0, error
         assert len(found) == len(kernels) and all(k in l.kernel for k, l in zip(kernels, found)), (call, found)
+
+
+def test_results_in_fp32_are_exact_products():
+    """Of any size, dense and by expert, but for what becomes codes: kernels whose last choice is the exact one."""
+    calls = [product(m, n, k, F32, offset) for m in (1, 40, 300, 8001) for n, k in ((512, 512), (6144, 4096), (6150, 4096), (6144, 640)) for offset in (0, 1)]
+    calls += [experts_product(8, rows, 4096, k, F32, gated) for rows in (1, 64, 400, 1000, 9000) for k in (512, 656, 4099) for gated in (0, 1)]
+    for call, (status, error, found) in zip(calls, launches(*calls)):
+        assert status == 0, error
+        products = [l for l in found if "finish" not in l.kernel]
+        assert products and all("true>(" in l.kernel for l in products), (call, found)
