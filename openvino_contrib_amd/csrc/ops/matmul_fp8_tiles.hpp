@@ -36,7 +36,7 @@ __global__ __launch_bounds__(64 * kWM * kWN) __attribute__((amdgpu_waves_per_eu(
     constexpr int kLoads = kRows / kRowsPerLoad / kWaves;  // of a wavefront for a stage, and one more of scales
     // behind a stage's rows: the activations' scales (64 lanes at a time), the weights' two, and room for the wavefronts that have none to load
     constexpr int kScaleWaves = (kBM + 63) / 64, kScalesAt = kRows * kStageBytes, kSlot = kScalesAt + 256 * (kScaleWaves + 2);
-    static_assert(kBN == kFp8Block, "of a gated unit: 64 columns of each half");
+    static_assert(kBN == kFp8Block, "a block of scales; of a gated unit: 64 columns of each half");
     static_assert(kRows % (kRowsPerLoad * kWaves) == 0 && kBM % kRowsPerLoad == 0 && kTM > 0 && kTN > 1 && kTN % 2 == 0, "whole loads and tiles");
     static_assert(kRing >= 2 && (kDirect || kRing == 2) && kWaves > kScaleWaves, "the stage that is read, and those on their way");
     constexpr int kOutColumns = 16 * kTN, kOutRow = 4 * kOutColumns + 16, kOutBytes = 16 * kOutRow;
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(64 * kWM * kWN) __attribute__((amdgpu_waves_per_eu(
         else
             source[i] = (weights ? b0 : a0) + from;
     }
-    // scales: wavefronts 0 .. kScaleWaves - 1 those of 64 activation rows each, the next the weights' of the tile's two halves, the others the same for nothing
+    // scales: wavefronts 0 .. kScaleWaves - 1 those of 64 activation rows each, the next the weights' (gated: of the two halves in turn), the others the same for nothing
     const int64_t blocks = stages, n_blocks = (p.n + kFp8Block - 1) / kFp8Block;
     const uint8_t* scale_at;
     int64_t scale_step;
@@ -121,8 +121,7 @@ __global__ __launch_bounds__(64 * kWM * kWN) __attribute__((amdgpu_waves_per_eu(
         scale_at = (const uint8_t*)(p.a_scales + activation_row(min(64 * wave + lane, kBM - 1)) * p.a_scale_row);
         scale_step = 4 * p.a_scale_block;
     } else {
-        const int half = lane & 1;
-        const int64_t row = p.gated ? (half ? up : gate) + n0 : min(n0 + half * (kBN / 2), p.n - 1);
+        const int64_t row = p.gated ? (lane & 1 ? up : gate) + n0 : n0;  // (a tile's columns share a block; of a gated unit, each half of them)
         scale_at = (const uint8_t*)(p.b_scales + ((int64_t)expert * n_blocks + row / kFp8Block) * blocks);
         scale_step = 4;
     }
@@ -176,9 +175,7 @@ __global__ __launch_bounds__(64 * kWM * kWN) __attribute__((amdgpu_waves_per_eu(
                 for (int e = 0; e < 8; e++) w[j][e] = (e < 4 ? quarter : quarter + 4) >= tail ? 0 : w[j][e];
             }
         }
-        // (columns of one wavefront share a block; of a gated unit, each half of them)
-        const int second = !p.gated && kBN > kFp8Block && (wn - kBM) >= kBN / 2;
-        const float scale_lo = scales[64 * kScaleWaves + second], scale_hi = p.gated ? scales[64 * kScaleWaves + 1] : scale_lo;
+        const float scale_lo = scales[64 * kScaleWaves], scale_hi = scales[64 * kScaleWaves + 1];
         float a_scale[kTM];
 #pragma unroll
         for (int i = 0; i < kTM; i++) a_scale[i] = scales[wm + 16 * i + frow];
@@ -311,17 +308,21 @@ __global__ __launch_bounds__(256) void matmul_fp8_finish_kernel(MatmulFp8Params 
 }
 
 template <int kBM, int kBN, int kWM, int kWN, int kRing, bool kDirect, bool kExperts>
-void launch(const MatmulFp8Params& p, Fp8Grid g, bool exact, hipStream_t stream) {
+hipError_t launch(const MatmulFp8Params& p, Fp8Grid g, bool exact, hipStream_t stream) {
     const int64_t tiles_m = kExperts ? most_expert_tiles(p, kBM) : (p.m + kBM - 1) / kBM;
     g.tiles_m = (int)tiles_m;
     g.tiles_n = (int)(p.gated ? GatedTiles(p.n / 2).count() : (p.n + kBN - 1) / kBN);
     g.rotate = !kExperts && tiles_m == 1 && g.parts == 1;
     const int64_t grid = 8 * ((tiles_m * g.tiles_n * g.parts + 7) / 8);
-    constexpr bool kToo = kBM == 32 || kBM == 128;  // (results in fp32: tiles of these sizes alone)
-    if (exact)
-        hipLaunchKernelGGL((matmul_fp8_tiles_kernel<kBM, kBN, kWM, kWN, kRing, kDirect, kExperts, kToo>), dim3((unsigned)grid), dim3(64 * kWM * kWN), 0, stream, p, g);
-    else
-        hipLaunchKernelGGL((matmul_fp8_tiles_kernel<kBM, kBN, kWM, kWN, kRing, kDirect, kExperts, false>), dim3((unsigned)grid), dim3(64 * kWM * kWN), 0, stream, p, g);
+    const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * kWM * kWN), 0, stream, p, g); };
+    if (!exact) {
+        run(matmul_fp8_tiles_kernel<kBM, kBN, kWM, kWN, kRing, kDirect, kExperts, false>);
+    } else if constexpr (kBM == 32 || kBM == 128) {  // (results in fp32: tiles of these sizes alone)
+        run(matmul_fp8_tiles_kernel<kBM, kBN, kWM, kWN, kRing, kDirect, kExperts, true>);
+    } else {
+        return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -333,18 +334,18 @@ hipError_t launch_matmul_fp8_tiles(const MatmulFp8Params& p, const Fp8Plan& plan
     g.group_rows = 8;
     g.sums_stride = (p.n + 3) / 4 * 4;
     if (plan.parts > 1) g.sums = (float*)workspace;
+    hipError_t e = hipSuccess;
     switch (plan.tile) {
         case kFp8Few: return launch_matmul_fp8_few<kExperts>(p, exact, stream);
         case kFp8Tile256: return launch_matmul_fp8_deep<kExperts>(p, stream);
-        case kFp8Tile128: launch<128, 128, 2, 2, 2, true, kExperts>(p, g, exact, stream); break;
+        case kFp8Tile128: e = launch<128, 128, 2, 2, 2, true, kExperts>(p, g, exact, stream); break;
         // (eight wavefronts where a compute unit has one or two workgroups, as a rule of dense products: 256 x 8,192 x 4,096 25.0 -> 21.2 us, 64 x 28,672 x
         // 4,096 31.0 -> 28.8; experts' many small tiles want room for more workgroups: 8 experts of 28,672 x 4,096 with 32 rows each 194 us, with eight 235)
-        case kFp8Tile64: launch<64, 128, kExperts ? 1 : 2, 4, 3, true, kExperts>(p, g, exact, stream); break;
-        case kFp8Tile32: launch<32, 128, 1, 4, 3, true, kExperts>(p, g, exact, stream); break;
-        case kFp8Any128: launch<128, 128, 2, 4, 2, false, kExperts>(p, g, exact, stream); break;
-        default: launch<32, 128, 1, 4, 2, false, kExperts>(p, g, exact, stream); break;
+        case kFp8Tile64: e = launch<64, 128, kExperts ? 1 : 2, 4, 3, true, kExperts>(p, g, exact, stream); break;
+        case kFp8Tile32: e = launch<32, 128, 1, 4, 3, true, kExperts>(p, g, exact, stream); break;
+        case kFp8Any128: e = launch<128, 128, 2, 4, 2, false, kExperts>(p, g, exact, stream); break;
+        default: e = launch<32, 128, 1, 4, 2, false, kExperts>(p, g, exact, stream); break;
     }
-    hipError_t e = hipGetLastError();
     if (e != hipSuccess || plan.parts == 1) return e;
     hipLaunchKernelGGL(matmul_fp8_finish_kernel, dim3((unsigned)((p.n + 1023) / 1024), (unsigned)p.m), dim3(256), 0, stream, p, g.sums, g.sums_stride, g.parts);
     return hipGetLastError();
