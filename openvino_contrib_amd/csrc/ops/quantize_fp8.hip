@@ -286,7 +286,7 @@ hipattn_status quantize_fp8(const hipops_quantize_fp8_desc* d, const void* x, co
         return fail(HIPATTN_INVALID_ARGUMENT, "quantize_fp8: rows of %lld elements, %lld apart", (long long)taken, (long long)d->x_row_stride);
     const int64_t row = d->scale_row_stride, block = d->scale_block_stride;
     if (row > (int64_t)1 << 40 || block > (int64_t)1 << 40) return fail(HIPATTN_UNSUPPORTED, "quantize_fp8: scales %lld and %lld apart", (long long)row, (long long)block);
-    if (row < 0 || block < 0 || ((row == 0) != (block == 0)) || (row && !(row >= blocks * block || block >= d->rows * row)))
+    if (row < 0 || block < 0 || ((row == 0) != (block == 0)) || (row && !(row >= blocks * block || block / row >= d->rows)))
         return fail(HIPATTN_INVALID_ARGUMENT, "quantize_fp8: scales of %lld rows and %lld blocks overlap, %lld and %lld apart", (long long)d->rows, (long long)blocks,
                     (long long)row, (long long)block);
     if (d->rows == 0) return HIPATTN_OK;

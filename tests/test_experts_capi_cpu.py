@@ -67,6 +67,13 @@ def test_quantise_refusals():
     call("null pointer", x=None)
 
 
+def test_quantise_refuses_scales_that_overlap_however_far_apart():
+    """rows x stride beyond 2^63: columns' scales 2^39 and rows' 2^40 apart fall onto one another."""
+    for rows, row, block, width in ((1 << 23, 1 << 40, 1 << 39, 384), ((1 << 31) - 1, 1 << 40, 1 << 40, 256), (1 << 24, 1 << 40, 1 << 40, 256)):
+        d = ops_capi.QuantizeFp8Desc(x_dtype=capi.F16, rows=rows, width=width, scale_row_stride=row, scale_block_stride=block)
+        refused("hipops_quantize_fp8", d, [P, P, P, P, None], "overlap")
+
+
 def test_product_refusals():
     def call(word, status=capi.INVALID_ARGUMENT, args=(P, P, P, P, None, None, P, None, 0, None), **fields):
         d = ops_capi.MatmulFp8Desc(c_dtype=capi.BF16, m=4, n=256, k=256)
