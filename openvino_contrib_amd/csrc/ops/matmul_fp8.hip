@@ -146,7 +146,7 @@ Fp8Tile expert_tile_of(const MatmulFp8Params& p, bool aligned, bool exact) {
 hipError_t launch_experts(const MatmulFp8Params& p, bool exact, hipStream_t stream) {
     // (tiles that load straight to LDS address rows in 32 bits: those of a from its beginning or the tile's, weights from the tile's first row)
     const int64_t limit = (int64_t)1 << 32;
-    const bool aligned = (((uintptr_t)p.a | (uintptr_t)p.b | (uintptr_t)p.lda | (uintptr_t)p.k) & 15) == 0 && (p.order ? p.a_rows : 256) * p.lda < limit &&
+    const bool aligned = (((uintptr_t)p.a | (uintptr_t)p.b | (uintptr_t)p.lda | (uintptr_t)p.k) & 15) == 0 && p.lda < limit && (p.order ? p.a_rows : 256) * p.lda < limit &&
                          (p.gated ? p.n : 256) * p.ldb < limit;
     return launch_matmul_fp8_tiles<true>(p, {expert_tile_of(p, aligned, exact), 1}, exact, nullptr, stream);
 }

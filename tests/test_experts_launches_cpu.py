@@ -115,3 +115,16 @@ def test_results_in_fp32_are_exact_products():
         assert status == 0, error
         products = [l for l in found if "finish" not in l.kernel]
         assert products and all("true>(" in l.kernel for l in products), (call, found)
+
+
+@pytest.mark.parametrize("a_rows,lda", [(50, 1 << 27), (1 << 20, 4096), ((1 << 31) - 1, 1 << 33), (1 << 24, 1 << 40), (1 << 30, 1 << 34)])
+def test_rows_of_experts_that_32_bits_do_not_reach(a_rows, lda):
+    """Rows named by an order go to the kernels with whole addresses as soon as one may lie 2^32 bytes behind the first, products that pass 64 bits included."""
+    calls = []
+    for rows in (4, 400, 4000):
+        call = experts_product(8, rows, 512, 512, BF16)
+        call[2].update(a_rows=a_rows, lda=lda)
+        calls.append(call)
+    for status, error, found in launches(*calls):
+        assert status == 0, error
+        assert len(found) == 1 and "matmul_fp8_tiles_kernel<" in found[0].kernel and found[0].kernel.split("<")[1].split(",")[5].strip() == "false", found
