@@ -134,6 +134,22 @@ def test_lists_of_one_sought_expert(hip, ops):  # noqa: F811
     check_routing(hip, ops, -logits, None, 1, score="sigmoid")
 
 
+@pytest.mark.parametrize("tokens", [8, 9, 1024, 1025, 4096, 4097, 32768, 32769, 1 << 18, (1 << 18) + 1, 700001])
+@pytest.mark.parametrize("experts,top_k", [(5, 2), (130, 3)])
+def test_lists_about_the_lengths_of_runs(hip, ops, tokens, experts, top_k):  # noqa: F811
+    """Every token chooses expert 3 (a run's count of it is the run's length, 224 at most), and others as they come."""
+    logits = np.random.default_rng(tokens).standard_normal((tokens, experts)).astype(np.float32)
+    logits[:, 3] = 9
+    (indices, weights, *found), _ = routed(hip, ops, logits, None, top_k)
+    want = np.argsort(-logits, 1, kind="stable")[:, :top_k]
+    assert np.array_equal(indices, want)
+    for got, ref in zip(found, R.lists(indices, experts)):
+        assert np.array_equal(got, ref)
+    y = np.exp(np.take_along_axis(logits, want, 1).astype(np.float64))
+    y /= y.sum(1, keepdims=True)
+    assert np.all(np.abs(weights - y) <= y * 2.0 ** -23)
+
+
 def test_routing_of_more_tokens_than_a_launch_takes(hip, ops):  # noqa: F811
     """224 tokens to a workgroup of 1,024 threads: 2^32 of those are passed, and the call (without lists) goes in two launches.  Rows of equal logits, some others
     about the launches' ends."""
@@ -351,6 +367,42 @@ def test_more_places_than_a_launch_takes(hip, ops, n, k, c_dtype, gated):  # noq
     slack = 1.13 * each[:, gate] * (np.abs(ref[:, pair]) + each[:, pair]) + np.abs(ref[:, gate]) * each[:, pair] + 2.0 ** -20 * np.abs(ref).max(1, keepdims=True) ** 2
     y = R.gated(ref, 0, 1)
     assert np.all(np.abs(got - y) <= slack + HALF_ULP[c_dtype] * np.abs(y) * 1.001 + 3e-8)
+
+
+@pytest.mark.parametrize("which", ["none", "few", "uneven", "large"])
+@pytest.mark.parametrize("n", [2, 130, 512])
+def test_experts_without_k(hip, ops, which, n):  # noqa: F811
+    """Sums of nothing are zeros, their units and codes too."""
+    counts = COUNTS[which]
+    rows, spare, E = sum(counts), 3, len(counts)
+    begins = hip.DeviceBuffer.from_numpy(np.concatenate([[0], np.cumsum(counts)]).astype(np.int32))
+    for c_dtype, gated in ((F32, 0), (BF16, 0), (F16, 1), (E4M3, 1)):
+        width = n // 2 if gated else n
+        size = 1 if c_dtype == E4M3 else hip.DTYPE_BYTES[c_dtype]
+        d = ops.MatmulFp8ExpertsDesc(c_dtype, gated, 0, 1, 1, E, rows + spare, n, 0, rows + spare)
+        out, scales = hip.DeviceBuffer((rows + spare) * width * size), hip.DeviceBuffer(4 * (rows + spare) * R.blocks(width))
+        out.fill(0x7E)
+        scales.fill(0x7E)
+        ws = hip.DeviceBuffer(max(16, ops.matmul_fp8_experts_workspace_size(d)))
+        ws.fill(0xA5)
+        ops.matmul_fp8_experts(d, None, None, None, None, begins, None, out, scales if c_dtype == E4M3 else None, ws)
+        got = out.download(np.uint8, (rows + spare, width * size))
+        assert not np.any(got[:rows] & 0x7F) and np.all(got[rows:] == 0x7E)
+        if c_dtype == E4M3:
+            s = scales.download(np.uint32, (R.blocks(width), rows + spare))
+            assert not s[:, :rows].any() and np.all(s[:, rows:] == 0x7E7E7E7E)
+
+
+@pytest.mark.parametrize("which", ["few", "uneven", "many", "large"])
+def test_experts_narrow_units_and_padded_rows(hip, ops, which):  # noqa: F811
+    """One result column; rows with something between them and scales by row, in the tiles of 256 rows too."""
+    for c_dtype in (BF16, F32):
+        check_experts(hip, ops, COUNTS[which], 2, 256, c_dtype, gated=True, tokens=37, top_k=3, spare=5)
+    check_experts(hip, ops, COUNTS[which], 2, 130, E4M3)
+    for pad in (16, 48, 64):
+        check_experts(hip, ops, COUNTS[which], 512, 1024, BF16, pad=pad, by_row=True)
+        check_experts(hip, ops, COUNTS[which], 512, 1024, E4M3, pad=pad, by_row=True, tokens=37, top_k=3, spare=5)
+        check_experts(hip, ops, COUNTS[which], 512, 1024, F16, gated=True, pad=pad, tokens=500)
 
 
 def test_many_experts(hip, ops):  # noqa: F811
