@@ -65,6 +65,8 @@ hipattn_status hipops_route_experts(const hipops_route_desc* desc, const void* l
  * c: [rows, n] of F32 / F16 / BF16, packed; where `gated` is set, [rows, n / 2]: the GLU of the halves of that row (glu_activation,
  * glu_gate_first as hipops_glu), in fp32 and rounded once.  c_dtype HIPOPS_F8_E4M3 (gated alone): that GLU as codes [rows, n / 2] with
  * c_scales [ceil(n / 2 / 128), rows], as hipops_quantize_fp8 leaves them: the rows of the next product.  c_scales is not looked at otherwise.
+ * F32 results are sums of exact products; those of 16 bits, and the fp32 values that become codes, come from the 8-bit matrix instruction and
+ * are about 1.4e-5 off in the 2-norm on normal operands (hipops_fp8.h), ahead of a code's rounding of 2^-4 of the value at most.
  * The workspace holds what hipops_matmul_fp8_experts_workspace_size asks for.  The same call gives the same bits every time. */
 typedef struct hipops_matmul_fp8_experts_desc {
     int c_dtype;

@@ -160,7 +160,8 @@ __device__ __forceinline__ Float8 float8_of(const Raw8& r, int dtype) {
     return y;
 }
 
-// swish with the reciprocal instruction, good to a unit in the last place
+// swish with the exponential and the reciprocal instruction: a unit in the last place off each, and the exponent x log2 e is rounded to 24 bits: for negative x
+// some (1.2 |x| + 8) 2^-24 of the value, which is |x| exp(-|x|) there
 __device__ __forceinline__ float gated(float x, int activation) {
     if (activation == HIPOPS_GLU_SWISH) return x * __builtin_amdgcn_rcpf(1.0f + __expf(-x));
     return activate(x, activation, 1.0f);
