@@ -141,6 +141,22 @@ def test_quantise_strides_and_alignment(hip, ops):  # noqa: F811
             assert np.all(np.abs(R.VALUES[codes] - R.VALUES[plain]) <= np.maximum(np.abs(R.VALUES[plain]) / 8, 2.0 ** -9) * 1.01)
 
 
+@pytest.mark.parametrize("width", [1 << 24, (1 << 24) + 129])
+@pytest.mark.parametrize("source", [0, 2])
+def test_quantise_the_widest_rows(hip, ops, width, source):  # noqa: F811
+    """A row's workgroups fill the grid's second dimension half, and wider rows take a workgroup each: 64 blocks over and over have the same codes every time."""
+    rng = np.random.default_rng(width)
+    halves = [rng.standard_normal((3, 8192)).astype(np.float32) for _ in range(2 if source == 2 else 1)]
+    want, want_scales, _, _ = quantised(hip, ops, np.concatenate(halves, 1), F16, source)
+    wide = lambda x, n: np.tile(x, (1, -(-n // x.shape[1])))[:, :n]
+    codes, scales, _, _ = quantised(hip, ops, np.concatenate([wide(h, width) for h in halves], 1), F16, source)
+    whole = width // 128
+    assert np.array_equal(codes[:, :whole * 128], wide(want, whole * 128)) and np.array_equal(scales[:, :whole], wide(want_scales, whole))
+    if width % 128:  # (a single column in the last block)
+        assert width % 128 == 1 and np.array_equal(R.VALUES[codes[:, -1]], np.sign(R.VALUES[codes[:, -1]]) * 448.0)
+        assert np.array_equal(np.sign(R.VALUES[codes[:, -1]]), np.sign(R.VALUES[want[:, whole * 128 % 8192]]))
+
+
 def test_a_block_of_infinities_leaves_the_others(hip, ops):  # noqa: F811
     x = np.random.default_rng(3).standard_normal((4, 512)).astype(np.float32)
     want = quantised(hip, ops, x, F16)
